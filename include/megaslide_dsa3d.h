@@ -11,7 +11,10 @@
  *     offset_net[0:2] = depthwise 3x3x3 conv + GELU (attention.py:71-72, :105)
  *     and their backward                             -> msd_dwconv3d_fwd / _bwd
  * The Linear projections and the 1x1 offset conv stay dense GEMMs in the host
- * framework.
+ * framework.  Beside it, for layers that attend densely (the reference's global
+ * attention, infinity/video/baselines.py): the norm of queries and keys with the
+ * rotation by their positions (msd_qk_rope_*) and attention over packed sequences
+ * (msd_attn_*).
  *
  * Conventions
  *   - Tensors are channel-last: token n = (t*H + h)*W + w, as the reference
@@ -109,6 +112,47 @@ typedef struct msd_dwconv3d_desc {
   int32_t dtype;               /* msd_dtype of x, y, weight, bias and grads       */
   int32_t act;                 /* 0 = none, 1 = exact-erf GELU after the bias     */
 } msd_dwconv3d_desc;
+
+/* Type of the positions of msd_qk_rope_*. */
+typedef enum msd_pos_dtype {
+  MSD_POS_I32 = 0, MSD_POS_I64 = 1, MSD_POS_F32 = 2, MSD_POS_F64 = 3,
+  MSD_POS_GRID = 4             /* no tensor: (t, h, w) of a video grid's tokens   */
+} msd_pos_dtype;
+
+/* Shape and options of one rotation (and norm) of queries and keys. */
+typedef struct msd_qk_rope_desc {
+  int64_t tokens;              /* rows of q and k                                 */
+  int64_t pos_rows;            /* rows of positions: token i has row i mod pos_rows */
+  int64_t q_stride, k_stride;  /* elements between consecutive tokens             */
+  double theta;                /* base of the frequencies, > 0                    */
+  int32_t q_heads, k_heads;    /* k_heads may be 0: q alone                       */
+  int32_t head_dim;            /* 2 to 256                                        */
+  int32_t dtype;               /* msd_dtype of q, k, results and their gradients  */
+  int32_t weight_dtype;        /* msd_dtype of the norm's weights and their gradients:
+                                  MSD_F32, or that of q                           */
+  int32_t pos_dtype;           /* msd_pos_dtype                                   */
+  int32_t n_axes;              /* 1 to 4: columns of positions (3 with a grid)    */
+  int32_t axis_dims[4];        /* channels turned by each axis: even, >= 0, sum <=
+                                  head_dim; channels behind them pass through     */
+  int32_t interleaved;         /* 1: pairs (2i, 2i+1) of an axis's channels; 0:
+                                  (i, i + d/2)                                    */
+  int32_t norm;                /* 1: RMS norm of each head before the rotation    */
+  float eps;                   /* the norm's                                      */
+  int32_t grid[3];             /* T, H, W of MSD_POS_GRID, pos_rows = T*H*W        */
+} msd_qk_rope_desc;
+
+/* Shape and options of attention over packed sequences. */
+typedef struct msd_attn_desc {
+  int64_t total_q, total_k;    /* rows of q, and of k and v, in all sequences     */
+  int64_t q_stride, k_stride, v_stride;  /* elements between consecutive rows     */
+  int32_t num_seqs;            /* >= 1                                            */
+  int32_t num_heads;           /* query heads, a multiple of num_kv_heads         */
+  int32_t num_kv_heads;
+  int32_t head_dim;            /* 1 to 128                                        */
+  int32_t dtype;               /* msd_dtype                                       */
+  int32_t causal;              /* 1: query i of lq sees keys j <= i + lk - lq     */
+  float scale;                 /* of the scores, finite and > 0                   */
+} msd_attn_desc;
 
 /* Version of this header's ABI (MSD_ABI_VERSION). */
 int msd_abi_version(void);
@@ -216,6 +260,69 @@ int msd_dwconv3d_bwd(const msd_dwconv3d_desc* desc, const void* x, const void* w
                      const void* bias, const void* preact, const void* dy, void* dx,
                      void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/*
+ * Rotation of queries and keys by their tokens' positions on several axes, after
+ * an RMS norm of each head where desc->norm is set, in one pass:
+ *   y = R(pos) (w * x / sqrt(mean(x^2) + eps))
+ * Pair i of axis a (d_a channels) turns by pos_a * theta^(-2 i / d_a), an angle
+ * held in 64 bits.  q [tokens, q_heads*head_dim] and k with their strides;
+ * q_out, k_out contiguous.  positions [pos_rows, n_axes] contiguous (NULL
+ * with MSD_POS_GRID: token n = (t*H + h)*W + w).  q_weight, k_weight [head_dim],
+ * NULL for ones.  k and k_out are NULL when k_heads = 0.
+ */
+int msd_qk_rope_fwd(const msd_qk_rope_desc* desc, const void* q, const void* k,
+                    const void* q_weight, const void* k_weight, const void* positions,
+                    void* q_out, void* k_out, void* stream);
+
+/* Bytes of device workspace msd_qk_rope_bwd needs for `desc` (0 without the norm). */
+size_t msd_qk_rope_bwd_workspace_size(const msd_qk_rope_desc* desc);
+
+/*
+ * Backward of msd_qk_rope_fwd: dq_out, dk_out are the gradients of its results,
+ * dq, dk those of q and k (all contiguous; dq, dk written), dq_weight, dk_weight
+ * those of the weights (NULL when not wanted, and without the norm).  q and k are
+ * read with the norm only (else they may be NULL).  Sums are taken in a fixed
+ * order: results repeat bit for bit.
+ */
+int msd_qk_rope_bwd(const msd_qk_rope_desc* desc, const void* q, const void* k,
+                    const void* q_weight, const void* k_weight, const void* positions,
+                    const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight,
+                    void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace msd_attn_fwd needs for `desc` (0 where the keys are not split). */
+size_t msd_attn_fwd_workspace_size(const msd_attn_desc* desc);
+
+/*
+ * Attention over packed sequences with grouped heads:
+ *   out = softmax(scale q k^T + mask) v  of each sequence and head.
+ * Query head h reads key head h / (num_heads / num_kv_heads).  cu_q, cu_k
+ * [num_seqs + 1] int32: sequence s has rows cu[s] .. cu[s+1] - 1 of q (k, v); they
+ * begin with 0, do not fall and end at most at the totals.  Rows behind the last
+ * sequence get out = 0 and lse = -inf.  Both NULL: sequences of equal length
+ * total / num_seqs.  A row that sees no key has out = 0 and lse = -inf.
+ * q [total_q, num_heads*head_dim], k, v [total_k, num_kv_heads*head_dim] with their
+ * strides; out [total_q, num_heads*head_dim] contiguous; lse [total_q, num_heads]
+ * fp32 or NULL.  What a row does not see (other sequences, later keys) does not
+ * change it, infinities and NaN there included.
+ */
+int msd_attn_fwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
+                 const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace msd_attn_bwd needs for `desc`. */
+size_t msd_attn_bwd_workspace_size(const msd_attn_desc* desc);
+
+/*
+ * Backward of msd_attn_fwd: out and lse are its results, dout (contiguous) the
+ * gradient of out, dlse [total_q, num_heads] fp32 that of lse (NULL = 0).  dq, dk,
+ * dv are written, contiguous; rows in no sequence get zeros.  Sums are taken in a
+ * fixed order: results repeat bit for bit.
+ */
+int msd_attn_bwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
+                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* dout,
+                 const float* lse, const float* dlse, void* dq, void* dk, void* dv,
+                 void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

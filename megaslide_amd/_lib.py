@@ -36,6 +36,13 @@ EXPORTS = (
     "msd_dwconv3d_fwd",
     "msd_dwconv3d_bwd_workspace_size",
     "msd_dwconv3d_bwd",
+    "msd_qk_rope_fwd",
+    "msd_qk_rope_bwd_workspace_size",
+    "msd_qk_rope_bwd",
+    "msd_attn_fwd_workspace_size",
+    "msd_attn_fwd",
+    "msd_attn_bwd_workspace_size",
+    "msd_attn_bwd",
 )
 
 
@@ -68,6 +75,36 @@ class ConvDesc(ctypes.Structure):
         ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("H", ctypes.c_int32), ("W", ctypes.c_int32),
         ("C", ctypes.c_int32), ("kt", ctypes.c_int32), ("kh", ctypes.c_int32), ("kw", ctypes.c_int32),
         ("dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+    ]
+
+
+class QkRopeDesc(ctypes.Structure):
+    """msd_qk_rope_desc."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("pos_rows", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("theta", ctypes.c_double),
+        ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("pos_dtype", ctypes.c_int32),
+        ("n_axes", ctypes.c_int32), ("axis_dims", ctypes.c_int32 * 4),
+        ("interleaved", ctypes.c_int32), ("norm", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("grid", ctypes.c_int32 * 3),
+    ]
+
+
+POS_DTYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+POS_GRID = 4
+
+
+class AttnDesc(ctypes.Structure):
+    """msd_attn_desc."""
+
+    _fields_ = [
+        ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64), ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("num_seqs", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -110,6 +147,22 @@ def load() -> ctypes.CDLL:
         lib.msd_dwconv3d_bwd_workspace_size.argtypes = [ctypes.POINTER(ConvDesc)]
         lib.msd_dwconv3d_bwd.restype = ctypes.c_int
         lib.msd_dwconv3d_bwd.argtypes = [ctypes.POINTER(ConvDesc)] + [_vp] * 9 + [ctypes.c_size_t, _vp]
+        lib.msd_qk_rope_fwd.restype = ctypes.c_int
+        lib.msd_qk_rope_fwd.argtypes = [ctypes.POINTER(QkRopeDesc)] + [_vp] * 8
+        lib.msd_qk_rope_bwd_workspace_size.restype = ctypes.c_size_t
+        lib.msd_qk_rope_bwd_workspace_size.argtypes = [ctypes.POINTER(QkRopeDesc)]
+        lib.msd_qk_rope_bwd.restype = ctypes.c_int
+        lib.msd_qk_rope_bwd.argtypes = ([ctypes.POINTER(QkRopeDesc)] + [_vp] * 12 +
+                                        [ctypes.c_size_t, _vp])
+        lib.msd_attn_fwd_workspace_size.restype = ctypes.c_size_t
+        lib.msd_attn_fwd_workspace_size.argtypes = [ctypes.POINTER(AttnDesc)]
+        lib.msd_attn_fwd.restype = ctypes.c_int
+        lib.msd_attn_fwd.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 8 + [ctypes.c_size_t, _vp]
+        lib.msd_attn_bwd_workspace_size.restype = ctypes.c_size_t
+        lib.msd_attn_bwd_workspace_size.argtypes = [ctypes.POINTER(AttnDesc)]
+        lib.msd_attn_bwd.restype = ctypes.c_int
+        lib.msd_attn_bwd.argtypes = ([ctypes.POINTER(AttnDesc)] + [_vp] * 13 +
+                                     [ctypes.c_size_t, _vp])
         v = lib.msd_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError(f"megaslide_amd: library ABI {v}, bindings expect {ABI_VERSION}")

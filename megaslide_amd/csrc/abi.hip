@@ -5,7 +5,9 @@
 
 #include <mutex>
 
+#include "attn.h"
 #include "common.h"
+#include "qk_rope.h"
 
 namespace {
 
@@ -89,6 +91,93 @@ int check_conv(const msd_dwconv3d_desc* d) {
   if (d->dtype != MSD_F32 && d->dtype != MSD_BF16)
     return fail(MSD_ERR_UNSUPPORTED, "dwconv3d: dtype %d not supported", d->dtype);
   if (d->act != 0 && d->act != 1) return fail(MSD_ERR_UNSUPPORTED, "dwconv3d: act %d", d->act);
+  return MSD_OK;
+}
+
+int check_qk_rope(const msd_qk_rope_desc* d) {
+  if (d == nullptr) return fail(MSD_ERR_ARG, "qk_rope: desc is NULL");
+  if (d->tokens < 0 || d->tokens > (int64_t(1) << 40) || d->pos_rows < (d->tokens > 0 ? 1 : 0))
+    return fail(MSD_ERR_ARG, "qk_rope: bad sizes tokens=%lld pos_rows=%lld", (long long)d->tokens,
+                (long long)d->pos_rows);
+  if (d->q_heads < 1 || d->k_heads < 0 || d->q_heads > 65536 || d->k_heads > 65536)
+    return fail(MSD_ERR_ARG, "qk_rope: bad heads %d, %d", d->q_heads, d->k_heads);
+  if (d->head_dim < 2 || d->head_dim > 256)
+    return fail(MSD_ERR_UNSUPPORTED, "qk_rope: head_dim=%d outside [2, 256]", d->head_dim);
+  if (d->dtype != MSD_F32 && d->dtype != MSD_BF16)
+    return fail(MSD_ERR_UNSUPPORTED, "qk_rope: dtype %d not supported", d->dtype);
+  if (d->norm != 0 && d->norm != 1) return fail(MSD_ERR_ARG, "qk_rope: norm %d", d->norm);
+  if (d->norm && d->weight_dtype != MSD_F32 && d->weight_dtype != d->dtype)
+    return fail(MSD_ERR_UNSUPPORTED, "qk_rope: weight_dtype %d with dtype %d", d->weight_dtype,
+                d->dtype);
+  if (d->pos_dtype < MSD_POS_I32 || d->pos_dtype > MSD_POS_GRID)
+    return fail(MSD_ERR_UNSUPPORTED, "qk_rope: pos_dtype %d not supported", d->pos_dtype);
+  if (d->n_axes < 1 || d->n_axes > 4)
+    return fail(MSD_ERR_ARG, "qk_rope: %d axes outside [1, 4]", d->n_axes);
+  if (d->pos_dtype == MSD_POS_GRID &&
+      (d->n_axes != 3 || d->grid[0] < 1 || d->grid[1] < 1 || d->grid[2] < 1 ||
+       d->pos_rows / d->grid[0] / d->grid[1] != d->grid[2] ||
+       d->pos_rows % d->grid[0] != 0 || d->pos_rows / d->grid[0] % d->grid[1] != 0))
+    return fail(MSD_ERR_ARG, "qk_rope: grid (%d, %d, %d) needs 3 axes and as many position rows",
+                d->grid[0], d->grid[1], d->grid[2]);
+  int64_t sum = 0;
+  for (int x = 0; x < d->n_axes; ++x) {
+    if (d->axis_dims[x] < 0 || d->axis_dims[x] % 2 != 0)
+      return fail(MSD_ERR_ARG, "qk_rope: axis %d has %d channels (must be even)", x,
+                  d->axis_dims[x]);
+    sum += d->axis_dims[x];
+  }
+  if (sum > d->head_dim)
+    return fail(MSD_ERR_ARG, "qk_rope: the axes' %lld channels exceed head_dim=%d", (long long)sum,
+                d->head_dim);
+  if (!(d->theta > 0.0) || !std::isfinite(d->theta))
+    return fail(MSD_ERR_ARG, "qk_rope: theta %g must be finite and > 0", d->theta);
+  if (d->norm && (!(d->eps >= 0.0f) || !std::isfinite(d->eps)))
+    return fail(MSD_ERR_ARG, "qk_rope: eps %g must be finite and >= 0",
+                static_cast<double>(d->eps));
+  if (d->q_stride < static_cast<int64_t>(d->q_heads) * d->head_dim ||
+      d->k_stride < static_cast<int64_t>(d->k_heads) * d->head_dim)
+    return fail(MSD_ERR_ARG, "qk_rope: token strides (%lld, %lld) below heads*head_dim",
+                (long long)d->q_stride, (long long)d->k_stride);
+  return MSD_OK;
+}
+
+int check_attn(const msd_attn_desc* d) {
+  if (d == nullptr) return fail(MSD_ERR_ARG, "attn: desc is NULL");
+  if (d->num_heads < 1 || d->num_kv_heads < 1 || d->num_heads % d->num_kv_heads != 0)
+    return fail(MSD_ERR_ARG, "attn: num_heads=%d must be a multiple of num_kv_heads=%d",
+                d->num_heads, d->num_kv_heads);
+  if (d->head_dim < 1 || d->head_dim > msd::attn_max_head_dim())
+    return fail(MSD_ERR_UNSUPPORTED, "attn: head_dim=%d outside [1, %d]", d->head_dim,
+                msd::attn_max_head_dim());
+  if (d->dtype != MSD_F32 && d->dtype != MSD_BF16)
+    return fail(MSD_ERR_UNSUPPORTED, "attn: dtype %d not supported", d->dtype);
+  if (d->causal != 0 && d->causal != 1) return fail(MSD_ERR_ARG, "attn: causal %d", d->causal);
+  if (d->num_seqs < 1) return fail(MSD_ERR_ARG, "attn: num_seqs=%d", d->num_seqs);
+  // row and workgroup counts are 32-bit
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (d->total_q < 0 || d->total_k < 0 || d->num_heads > 65536 || d->num_seqs > kMost / d->num_heads ||
+      d->total_q > kMost / d->num_heads || d->total_k > kMost / d->num_kv_heads)
+    return fail(MSD_ERR_ARG, "attn: sizes out of range (total_q=%lld, total_k=%lld, num_seqs=%d)",
+                (long long)d->total_q, (long long)d->total_k, d->num_seqs);
+  if (!(d->scale > 0.0f) || !std::isfinite(d->scale))
+    return fail(MSD_ERR_ARG, "attn: scale %g must be finite and > 0",
+                static_cast<double>(d->scale));
+  const int64_t dq = static_cast<int64_t>(d->num_heads) * d->head_dim;
+  const int64_t dk = static_cast<int64_t>(d->num_kv_heads) * d->head_dim;
+  if (d->q_stride < dq || d->k_stride < dk || d->v_stride < dk)
+    return fail(MSD_ERR_ARG, "attn: strides (%lld, %lld, %lld) below heads*head_dim",
+                (long long)d->q_stride, (long long)d->k_stride, (long long)d->v_stride);
+  return MSD_OK;
+}
+
+int check_lengths(const msd_attn_desc* d, const int32_t* cu_q, const int32_t* cu_k) {
+  if ((cu_q == nullptr) != (cu_k == nullptr))
+    return fail(MSD_ERR_ARG, "attn: cu_q and cu_k go together");
+  if (cu_q != nullptr && (!aligned(cu_q, 4) || !aligned(cu_k, 4)))
+    return fail(MSD_ERR_ALIGN, "attn: cu_q or cu_k not 4-byte aligned");
+  if (cu_q == nullptr && (d->total_q % d->num_seqs != 0 || d->total_k % d->num_seqs != 0))
+    return fail(MSD_ERR_ARG, "attn: totals %lld, %lld are no multiples of num_seqs=%d",
+                (long long)d->total_q, (long long)d->total_k, d->num_seqs);
   return MSD_OK;
 }
 
@@ -302,6 +391,121 @@ int msd_dwconv3d_bwd(const msd_dwconv3d_desc* desc, const void* x, const void* w
   return launch_status(msd::launch_dwconv3d_bwd(*desc, x, weight, bias, preact, dy, dx, dweight,
                                                 dbias, workspace, static_cast<hipStream_t>(stream)),
                        "dwconv3d_bwd");
+}
+
+int msd_qk_rope_fwd(const msd_qk_rope_desc* desc, const void* q, const void* k,
+                    const void* q_weight, const void* k_weight, const void* positions,
+                    void* q_out, void* k_out, void* stream) {
+  int rc = check_qk_rope(desc);
+  if (rc != MSD_OK) return rc;
+  if (desc->tokens == 0) return MSD_OK;
+  const size_t a = elem_bytes(desc->dtype);
+  rc = check_ptrs("qk_rope_fwd", a, {q, q_out});
+  if (rc == MSD_OK && desc->k_heads > 0) rc = check_ptrs("qk_rope_fwd(k)", a, {k, k_out});
+  if (rc == MSD_OK && desc->pos_dtype != MSD_POS_GRID)
+    rc = check_ptrs("qk_rope_fwd(positions)", desc->pos_dtype & 1 ? 8 : 4, {positions});
+  if (rc != MSD_OK) return rc;
+  for (const void* p : {q_weight, k_weight})
+    if (p != nullptr && !aligned(p, elem_bytes(desc->weight_dtype)))
+      return fail(MSD_ERR_ALIGN, "qk_rope_fwd: weight misaligned");
+  const msd::QkRopePtrs p{{q, k}, {q_weight, k_weight}, {}, {q_out, k_out}, {}, positions};
+  return launch_status(
+      msd::launch_qk_rope(*desc, p, false, nullptr, static_cast<hipStream_t>(stream)),
+      "qk_rope_fwd");
+}
+
+size_t msd_qk_rope_bwd_workspace_size(const msd_qk_rope_desc* desc) {
+  if (check_qk_rope(desc) != MSD_OK) return 0;
+  return msd::qk_rope_bwd_ws_bytes(*desc);
+}
+
+int msd_qk_rope_bwd(const msd_qk_rope_desc* desc, const void* q, const void* k,
+                    const void* q_weight, const void* k_weight, const void* positions,
+                    const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight,
+                    void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_qk_rope(desc);
+  if (rc != MSD_OK) return rc;
+  const size_t a = elem_bytes(desc->dtype);
+  if (desc->tokens > 0) {
+    rc = check_ptrs("qk_rope_bwd", a, {dq_out, dq});
+    if (rc == MSD_OK && desc->k_heads > 0) rc = check_ptrs("qk_rope_bwd(k)", a, {dk_out, dk});
+    if (rc == MSD_OK && desc->norm) rc = check_ptrs("qk_rope_bwd(q)", a, {q});
+    if (rc == MSD_OK && desc->norm && desc->k_heads > 0)
+      rc = check_ptrs("qk_rope_bwd(k input)", a, {k});
+    if (rc == MSD_OK && desc->pos_dtype != MSD_POS_GRID)
+      rc = check_ptrs("qk_rope_bwd(positions)", desc->pos_dtype & 1 ? 8 : 4, {positions});
+    if (rc != MSD_OK) return rc;
+  }
+  for (const void* p : {q_weight, k_weight, static_cast<const void*>(dq_weight),
+                        static_cast<const void*>(dk_weight)})
+    if (p != nullptr && !aligned(p, elem_bytes(desc->weight_dtype)))
+      return fail(MSD_ERR_ALIGN, "qk_rope_bwd: weight misaligned");
+  const size_t need = msd::qk_rope_bwd_ws_bytes(*desc);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(MSD_ERR_WORKSPACE,
+                "qk_rope_bwd: workspace of %zu bytes (16-aligned) needed, got %zu", need,
+                workspace == nullptr ? size_t(0) : workspace_bytes);
+  const msd::QkRopePtrs p{{q, k}, {q_weight, k_weight}, {dq_out, dk_out}, {dq, dk},
+                          {dq_weight, dk_weight}, positions};
+  return launch_status(
+      msd::launch_qk_rope(*desc, p, true, workspace, static_cast<hipStream_t>(stream)),
+      "qk_rope_bwd");
+}
+
+size_t msd_attn_fwd_workspace_size(const msd_attn_desc* desc) {
+  if (check_attn(desc) != MSD_OK) return 0;
+  return msd::attn_fwd_ws_bytes(*desc);
+}
+
+int msd_attn_fwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
+                 const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  int rc = check_attn(desc);
+  if (rc == MSD_OK) rc = check_lengths(desc, cu_q, cu_k);
+  if (rc != MSD_OK) return rc;
+  if (desc->total_q == 0) return MSD_OK;
+  const size_t a = elem_bytes(desc->dtype);
+  rc = check_ptrs("attn_fwd", a, {q, out});
+  if (rc == MSD_OK && desc->total_k > 0) rc = check_ptrs("attn_fwd(k, v)", a, {k, v});
+  if (rc != MSD_OK) return rc;
+  if (lse != nullptr && !aligned(lse, 4)) return fail(MSD_ERR_ALIGN, "attn_fwd: lse misaligned");
+  const size_t need = msd::attn_fwd_ws_bytes(*desc);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(MSD_ERR_WORKSPACE, "attn_fwd: workspace of %zu bytes (16-aligned) needed, got %zu",
+                need, workspace == nullptr ? size_t(0) : workspace_bytes);
+  return launch_status(msd::launch_attn_fwd(*desc, msd::attn_args(*desc, q, k, v, cu_q, cu_k), out,
+                                            lse, workspace, static_cast<hipStream_t>(stream)),
+                       "attn_fwd");
+}
+
+size_t msd_attn_bwd_workspace_size(const msd_attn_desc* desc) {
+  if (check_attn(desc) != MSD_OK) return 0;
+  return msd::attn_bwd_ws_bytes(*desc);
+}
+
+int msd_attn_bwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
+                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* dout,
+                 const float* lse, const float* dlse, void* dq, void* dk, void* dv,
+                 void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_attn(desc);
+  if (rc == MSD_OK) rc = check_lengths(desc, cu_q, cu_k);
+  if (rc != MSD_OK) return rc;
+  const size_t a = elem_bytes(desc->dtype);
+  if (desc->total_q > 0) {
+    rc = check_ptrs("attn_bwd", a, {q, out, dout, dq});
+    if (rc == MSD_OK) rc = check_ptrs("attn_bwd(lse)", 4, {lse});
+  }
+  if (rc == MSD_OK && desc->total_k > 0) rc = check_ptrs("attn_bwd(k, v)", a, {k, v, dk, dv});
+  if (rc != MSD_OK) return rc;
+  if (dlse != nullptr && !aligned(dlse, 4)) return fail(MSD_ERR_ALIGN, "attn_bwd: dlse misaligned");
+  const size_t need = msd::attn_bwd_ws_bytes(*desc);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(MSD_ERR_WORKSPACE, "attn_bwd: workspace of %zu bytes (16-aligned) needed, got %zu",
+                need, workspace == nullptr ? size_t(0) : workspace_bytes);
+  const msd::AttnBwdPtrs p{out, dout, lse, dlse, dq, dk, dv};
+  return launch_status(msd::launch_attn_bwd(*desc, msd::attn_args(*desc, q, k, v, cu_q, cu_k), p,
+                                            workspace, static_cast<hipStream_t>(stream)),
+                       "attn_bwd");
 }
 
 }  // extern "C"

@@ -1,0 +1,398 @@
+// Device helpers of the packed attention kernels (attn_fwd.hip, attn_bwd.hip): which rows a
+// workgroup has, tiles in LDS, matrix-core fragments.
+//
+// All products are 32x32 blocks of the matrix cores.  A fragment is 8 consecutive values of the
+// summed index for one row (A) or column (B) a lane: lane l has row l % 32 and half g = l / 32
+// of 16 summed values (bf16: one instruction; fp32: eight, the same layout, since the order of
+// summed indexes is free as long as A and B agree).  A result block has column l % 32 in lane
+// l, rows 8 (r / 4) + 4 g + r % 4 in its 16 registers.  So a block of weights computed with its
+// queries (or keys) along the lanes is itself, rounded, a fragment of the next product over its
+// register rows: {4 g + 0..3, 8 + 4 g + 0..3} of each 16, and no lane exchanges anything.  The
+// other operand of that product is read from the row-major tile by transposing LDS reads.
+#pragma once
+
+#include "attn.h"
+#include "common.h"
+
+namespace msd {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634074f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// ---------------------------------------------------------------------------
+// element types
+// ---------------------------------------------------------------------------
+
+template <typename T>
+struct Elem;
+
+template <>
+struct Elem<bf16> {
+  typedef bf16x8 frag;
+  static constexpr int kPerChunk = 8;  // elements of 16 bytes
+};
+template <>
+struct Elem<float> {
+  typedef f32x8 frag;
+  static constexpr int kPerChunk = 4;
+};
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// Registers 8 t .. 8 t + 7 of a block of weights as a fragment (bf16: rounded to nearest even,
+// half a step of 2^-8 relative, the one rounding between the two products).
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::frag to_frag(const f32x16& s, int t) {
+  typename Elem<T>::frag r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (sizeof(T) == 2)
+      r[j] = static_cast<__bf16>(s[8 * t + j]);
+    else
+      r[j] = s[8 * t + j];
+  }
+  return r;
+}
+
+template <typename F>
+__device__ __forceinline__ F zero_frag() {
+  F r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = 0;
+  return r;
+}
+
+// Whether a fragment holds an infinity or NaN.
+__device__ __forceinline__ bool nonfinite(const bf16x8& f) {
+  const u32x4 u = __builtin_bit_cast(u32x4, f);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ bool nonfinite(const f32x8& f) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= (__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+
+// The fragment with infinities and NaN as zeros.
+template <typename F>
+__device__ __forceinline__ F finite_part(const F& f) {
+  F r = f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = static_cast<float>(f[j]);
+    if (!(fabsf(x) < INFINITY)) r[j] = 0;
+  }
+  return r;
+}
+
+// Maximum and sum of a value over the two halves of a wave (lanes l and l ^ 32).
+__device__ __forceinline__ float half_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // lower, upper half's
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---------------------------------------------------------------------------
+// sequences
+// ---------------------------------------------------------------------------
+
+struct Span {
+  int64_t q0, k0;  // first row of the sequence's queries and keys
+  int lq, lk;
+  int tile;        // tile of this workgroup within the sequence; < 0: no work
+};
+
+__device__ __forceinline__ int64_t bound_of(const int32_t* cu, int s, int64_t total) {
+  if (s == 0) return 0;
+  const int64_t c = cu[s];
+  return c < 0 ? 0 : (c > total ? total : c);
+}
+
+// The sequence and tile of work item `slot`, where a sequence of n rows (times `mul`) takes
+// tiles of `tile` rows.  Sequence s owns the slots from floor(mul cu[s] / tile) + s on: at least
+// as many as it has tiles, and their number is known on the host from the totals alone, so
+// lengths stay on the device.  Rows behind the last sequence make one more sequence without a
+// counterpart.  Offsets that are not in order or out of range give wrong rows, never rows
+// outside the tensors.  `keys`: tiles of keys, else of queries.
+__device__ __forceinline__ Span find_span(const AttnArgs& a, int64_t slot, int mul, int tile,
+                                          bool keys) {
+  Span r;
+  const int32_t* cu = keys ? a.cu_k : a.cu_q;
+  int s;
+  if (cu == nullptr) {
+    // equal lengths: the last tiles of all sequences first (the longest ones when causal)
+    const int n = keys ? a.nk : a.nq;
+    const int per = static_cast<int>((static_cast<int64_t>(n) * mul + tile - 1) / tile);
+    s = static_cast<int>(slot % a.seqs);
+    r.tile = per - 1 - static_cast<int>(slot / a.seqs);
+  } else {
+    const int64_t total = keys ? a.total_k : a.total_q;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.seqs + 1;  // the answer is in [lo, lo + n)
+    int64_t first = 0;           // its first slot
+    while (n > 1) {
+      const int step = (n + 63) / 64;
+      const int i = lane * step;
+      const bool in = i < n;
+      const int64_t c = in ? bound_of(cu, lo + i, total) * mul / tile + lo + i : 0;
+      const uint64_t ok = __ballot(in && c <= slot);
+      const int k = ok == 0 ? 0 : 63 - __builtin_clzll(ok);
+      first = __shfl(c, k);
+      lo += k * step;
+      n = n - k * step < step ? n - k * step : step;
+    }
+    s = __builtin_amdgcn_readfirstlane(lo);
+    r.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(slot - first));
+  }
+  const bool tail = s >= a.seqs;
+  if (a.cu_q != nullptr) {
+    r.q0 = tail && keys ? 0 : bound_of(a.cu_q, s, a.total_q);
+    int64_t e = tail ? (keys ? 0 : a.total_q) : bound_of(a.cu_q, s + 1, a.total_q);
+    r.lq = static_cast<int>(e > r.q0 ? e - r.q0 : 0);
+  } else {
+    r.q0 = static_cast<int64_t>(s) * a.nq;
+    r.lq = tail ? 0 : a.nq;
+  }
+  if (a.cu_k != nullptr) {
+    r.k0 = tail && !keys ? 0 : bound_of(a.cu_k, s, a.total_k);
+    int64_t e = tail ? (keys ? a.total_k : 0) : bound_of(a.cu_k, s + 1, a.total_k);
+    r.lk = static_cast<int>(e > r.k0 ? e - r.k0 : 0);
+  } else {
+    r.k0 = static_cast<int64_t>(s) * a.nk;
+    r.lk = tail ? 0 : a.nk;
+  }
+  r.q0 = (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(r.q0))));
+  r.k0 = (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(r.k0))));
+  r.lq = __builtin_amdgcn_readfirstlane(r.lq);
+  r.lk = __builtin_amdgcn_readfirstlane(r.lk);
+  const int64_t rows = static_cast<int64_t>(keys ? r.lk : r.lq) * mul;
+  if (r.tile < 0 || static_cast<int64_t>(r.tile) * tile >= rows) r.tile = -1;
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// tiles
+// ---------------------------------------------------------------------------
+
+// XOR of a row's 16-byte chunks.  bf16: eight rows at one chunk (16-byte reads) and four rows
+// at one pair of chunks (transposing reads) lie in different banks; even, so that a pair stays
+// a pair.  fp32: eight rows at one chunk do.
+template <typename T, int HD>
+__device__ __forceinline__ int swz(int row) {
+  if (sizeof(T) == 4) return row & 7;
+  if (HD == 128) return ((row & 3) << 2) | (((row >> 2) & 1) << 1);
+  if (HD == 64) return (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1);
+  return ((row >> 2) & 1) << 1;
+}
+
+// Element offset of channel c (a multiple of a chunk's) of a tile's row.
+template <typename T, int HD>
+__device__ __forceinline__ int at(int row, int c) {
+  constexpr int E = Elem<T>::kPerChunk;
+  return row * HD + (((c / E) ^ swz<T, HD>(row)) * E) + c % E;
+}
+
+// A tile of ROWS rows of HD channels on its way from memory to LDS, NT threads.  Rows at or
+// past `rows` and channels at or past hd become zeros.  VEC: 16-byte loads (aligned rows, hd a
+// multiple of a chunk).
+template <typename T, int HD, int ROWS, int NT, bool VEC>
+struct Tile {
+  static constexpr int E = Elem<T>::kPerChunk;
+  static constexpr int kChunks = HD / E;
+  static constexpr int kItems = (ROWS * kChunks + NT - 1) / NT;
+  u32x4 r[kItems];
+
+  template <typename RowPtr>
+  __device__ __forceinline__ void load(RowPtr row_ptr, int rows, int hd) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int item = threadIdx.x + i * NT;
+      const int row = item / kChunks, c = item % kChunks * E;
+      u32x4 v = {0, 0, 0, 0};
+      if (row < rows && row < ROWS && c < hd) {
+        const T* p = row_ptr(row) + c;
+        if (VEC) {
+          v = *reinterpret_cast<const u32x4*>(p);
+        } else if (sizeof(T) == 2) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (c + j < hd) v[j / 2] |= static_cast<uint32_t>(h[j]) << (16 * (j & 1));
+        } else {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < hd) v[j] = w[j];
+        }
+      }
+      r[i] = v;
+    }
+  }
+
+  __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int item = threadIdx.x + i * NT;
+      const int row = item / kChunks, c = item % kChunks * E;
+      if (ROWS * kChunks % NT == 0 || row < ROWS)
+        *reinterpret_cast<u32x4*>(lds + at<T, HD>(row, c)) = r[i];
+    }
+  }
+};
+
+// 8 channels c .. c + 7 (c a multiple of 8) of a tile's row.
+template <typename T, int HD>
+__device__ __forceinline__ typename Elem<T>::frag row_frag(const T* lds, int row, int c) {
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const bf16x8*>(lds + at<T, HD>(row, c));
+  } else {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(lds + at<T, HD>(row, c));
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(lds + at<T, HD>(row, c + 4));
+    return f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+}
+
+// Channel 32 blk + l % 32 of the tile's rows r0 + {4 g + 0..3, 8 + 4 g + 0..3} (r0 a multiple
+// of 16): the fragment that goes with to_frag's.
+template <typename T, int HD>
+__device__ __forceinline__ typename Elem<T>::frag col_frag(T* lds, int r0, int blk) {
+  const int l = threadIdx.x & 63, g = l >> 5;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) bf16x4 lds4;
+    const int row = r0 + 4 * g + ((l & 15) >> 2);
+    const int c = blk * 32 + ((l >> 4) & 1) * 16 + (l & 3) * 4;
+    const T* p = lds + at<T, HD>(row, c & ~7) + (c & 7);
+    // 8 rows further the XOR is the same
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + 8 * HD));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const int c = blk * 32 + (l & 31);
+    f32x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = r0 + (j / 4) * 8 + 4 * g + j % 4;
+      r[j] = lds[at<T, HD>(row, c & ~3) + (c & 3)];
+    }
+    return r;
+  }
+}
+
+// 8 channels of a row in memory, zeros at or past hd.
+template <typename T, bool VEC>
+__device__ __forceinline__ typename Elem<T>::frag mem_frag(const T* p, int c, int hd) {
+  typename Elem<T>::frag r = zero_frag<typename Elem<T>::frag>();
+  if (VEC) {
+    if (c < hd) {
+      if constexpr (sizeof(T) == 2) {
+        r = *reinterpret_cast<const bf16x8*>(p + c);
+      } else {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(p + c);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(p + c + 4);
+        r = f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (c + j < hd) {
+        if constexpr (sizeof(T) == 2)
+          r[j] = reinterpret_cast<const __bf16*>(p)[c + j];
+        else
+          r[j] = p[c + j];
+      }
+    }
+  }
+  return r;
+}
+
+// Stores block `blk` (32 channels) of a result with rows along the lanes: out[c] of the lane's
+// row, times f.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_block(T* out, const f32x16& acc, int blk, float f, int hd) {
+  const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = blk * 32 + 8 * i + 4 * g;
+    if (VEC) {
+      if (c < hd) {
+        if constexpr (sizeof(T) == 2) {
+          bf16x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = static_cast<__bf16>(acc[4 * i + j] * f);
+          *reinterpret_cast<bf16x4*>(out + c) = v;
+        } else {
+          *reinterpret_cast<f32x4*>(out + c) = f32x4{acc[4 * i] * f, acc[4 * i + 1] * f,
+                                                     acc[4 * i + 2] * f, acc[4 * i + 3] * f};
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < hd) out[c + j] = from_f32<T>(acc[4 * i + j] * f);
+    }
+  }
+}
+
+// Adds the infinities and NaN of an operand to a product whose weights are zero at masked
+// places, as the sum over the places that are not masked would have them: the product itself
+// was made with the operand's finite part, since 0 times infinity is NaN at masked places too.
+// w: weights (>= 0 or NaN), block of 32 summed rows x 32 lanes; seen(r): whether register row r
+// of the lane is not masked; frags(t): the operand's fragment of rows 16 t ...
+template <typename T, typename Seen, typename Frags>
+__device__ __forceinline__ void add_nonfinite(f32x16& acc, const f32x16& w, Seen seen,
+                                              Frags frags) {
+  typedef typename Elem<T>::frag F;
+#pragma unroll 1
+  for (int kind = 0; kind < 4; ++kind) {
+    // 0: +inf under a weight, 1: -inf under a weight, 2: NaN, 3: an infinity under weight zero
+    f32x16 n = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const F f = frags(t);
+      F ind = zero_frag<F>(), has = zero_frag<F>();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = static_cast<float>(f[j]), p = w[8 * t + j];
+        const bool i = kind == 0 ? x == INFINITY
+                       : kind == 1 ? x == -INFINITY
+                       : kind == 2 ? x != x
+                                   : fabsf(x) == INFINITY;
+        const bool h = seen(8 * t + j) && (kind == 2 || (kind == 3 ? p == 0.0f : p > 0.0f));
+        if (i) ind[j] = 1;
+        if (h) has[j] = 1;
+      }
+      n = mma(ind, has, n);
+    }
+    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (n[r] > 0.0f) acc[r] += add;
+  }
+}
+
+}  // namespace msd

@@ -258,7 +258,7 @@ def keep_core_policy(ctx, op, *args, **kwargs):
     kernel of the recompute, while the projections, convolutions and norms are
     rerun as usual."""
     from torch.utils.checkpoint import CheckpointPolicy
-    if op is torch.ops.megaslide.dsa3d_core.default:
+    if op in (torch.ops.megaslide.dsa3d_core.default, torch.ops.megaslide.packed_attention.default):
         return CheckpointPolicy.MUST_SAVE
     return CheckpointPolicy.PREFER_RECOMPUTE
 
@@ -277,7 +277,8 @@ def keep_gemms_policy(ctx, op, *args, **kwargs):
     the LayerNorms and the depthwise convolutions.  A DiT block at 46,800
     tokens, dim 1,536, then keeps ~2 GB of activations beyond its input."""
     from torch.utils.checkpoint import CheckpointPolicy
-    if op in (torch.ops.megaslide.dsa3d_core.default, torch.ops.aten.mm.default,
+    if op in (torch.ops.megaslide.dsa3d_core.default,
+              torch.ops.megaslide.packed_attention.default, torch.ops.aten.mm.default,
               torch.ops.aten.addmm.default):
         return CheckpointPolicy.MUST_SAVE
     return CheckpointPolicy.PREFER_RECOMPUTE
