@@ -7,22 +7,32 @@
 // axes pass through.  Backward, with g = R^T dy:
 //   dw = sum over rows of g x r,  dx = r (w g) - x r^3 mean(w g x)   (norm = 0: dx = R^T dy)
 //
-// Bound: memory.  x is read and y written once (backward: x, dy read, dx written).  A workgroup
-// takes a few tokens; it computes their cos and sin once into LDS (angles in revolutions, in
-// 64 bits, reduced to one turn before the 32-bit functions: positions of 10^6 lose nothing) and
-// then streams every head of q and of k past them, a row of 8-channel chunks per lane group,
-// 16 bytes a lane.  The partner of a channel is in the lane's own chunk (interleaved pairs) or
-// read through LDS (pairs half an axis apart, which no fixed shuffle serves for odd splits).
+// Bound: memory.  x is read and y written once (backward: x, dy read, dx written).  A wave takes
+// a token: its lanes compute the cos and sin of the token's pairs once into LDS (angles in
+// revolutions, in 64 bits, reduced to one turn before the 32-bit functions: positions of 10^6
+// lose nothing), each lane takes those of its 8 channels into registers, and the heads stream
+// past, a row per lane group, 16 bytes a lane, the next rows (the next token's after the last)
+// in flight meanwhile.  Workgroups of q and of k are apart: one tensor's weights fit the
+// registers beside two rows in flight.  The partner of a channel is in
+// the lane's own chunk (interleaved pairs) or read through LDS (pairs half an axis apart, which
+// no fixed shuffle serves for odd splits).  Where tokens are few, their heads are split among
+// workgroups.
 #include "common.h"
 #include "qk_rope.h"
+
+#include <type_traits>
 
 namespace msd {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTok = 8;     // tokens whose angles a workgroup holds at a time
 constexpr int kMaxPairs = 128;
-constexpr int kBwdBlocks = 1024;  // the weight gradient keeps one partial row per workgroup
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+// As many workgroups as the compute units hold at a time (the norm's backward, with one partial
+// row of the weights' gradients each, half as many): what a lane knows of its channels and the
+// weights is then set up once for many tokens.
+constexpr int kMaxBlocks = 2048;
+constexpr int kMaxBwdBlocks = 1024;
 
 struct RopeArgs {
   const void* x[2];        // q, k: rows of heads * hd channels, `stride` apart
@@ -34,11 +44,10 @@ struct RopeArgs {
   const void* pos;
   int64_t tokens, pos_rows;
   float* dw;               // [blocks][2][hd] partial sums of the weights' gradients, or null
-  int hd, n_axes, npairs, interleaved, pos_dtype, w_f32;
+  int hd, n_axes, npairs, pos_dtype, w_f32, pass;
   int axis[4];
   int grid[3];
   float eps;
-  int tok;                 // tokens of a workgroup's step
   double rev[kMaxPairs];   // revolutions per unit of position of each pair
 };
 
@@ -58,47 +67,70 @@ __device__ __forceinline__ double position(const RopeArgs& a, int64_t row, int x
   }
 }
 
-// Eight channels from c0 of a row; those at or past hd read as zero.  VEC: 16-byte loads, hd a
-// multiple of 8.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int c0, int hd, float (&v)[8]) {
-  if (VEC) {
-    if (c0 < hd) {
-      if (sizeof(T) == 2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p + c0);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight channels from c0 of a row as they are stored; those at or past hd are zeros.  VEC:
+// 16-byte loads, hd a multiple of 8.
+template <typename T>
+struct Raw {
+  uint4 u[sizeof(T) / 2];
+
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p, int c0, int hd, bool live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = __uint_as_float(w[i] << 16);
-          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-      } else {
-        const float4 lo = *reinterpret_cast<const float4*>(p + c0);
-        const float4 hi = *reinterpret_cast<const float4*>(p + c0 + 4);
-        v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-        v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) u[i] = make_uint4(0, 0, 0, 0);
+    if (!live) return;
+    if (VEC) {
+      if (c0 < hd) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+          u[i] = reinterpret_cast<const uint4*>(p + c0)[i];
       }
     } else {
+      union {
+        T e[8];
+        uint4 v[sizeof(T) / 2];
+      } x;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) x.v[i] = u[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < hd) x.e[i] = p[c0 + i];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) u[i] = x.v[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < hd ? to_f32(p[c0 + i]) : 0.0f;
   }
+
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_weight(const void* p, int c0, int hd, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c0 + i < hd ? to_f32(static_cast<const T*>(p)[c0 + i]) : 0.0f;
 }
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, int c0, int hd, const float (&v)[8]) {
   if (VEC) {
     if (c0 >= hd) return;
-    if (sizeof(T) == 2) {
-      uint32_t w[4];
+    if constexpr (sizeof(T) == 2) {
+      typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+      bf16x8 r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = static_cast<uint32_t>(from_f32<bf16>(v[2 * i]).bits) |
-               (static_cast<uint32_t>(from_f32<bf16>(v[2 * i + 1]).bits) << 16);
-      *reinterpret_cast<uint4*>(p + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int i = 0; i < 8; ++i) r[i] = static_cast<__bf16>(v[i]);
+      *reinterpret_cast<bf16x8*>(p + c0) = r;
     } else {
       *reinterpret_cast<float4*>(p + c0) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(p + c0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -110,235 +142,292 @@ __device__ __forceinline__ void store8(T* p, int c0, int hd, const float (&v)[8]
   }
 }
 
-// LPR: lanes of a row (8 channels each).
-template <typename T, int LPR, bool NORM, bool BWD, bool VEC>
-__global__ __launch_bounds__(kThreads) void qk_rope_kernel(const RopeArgs a) {
-  constexpr int kGroups = kThreads / LPR;
-  __shared__ float2 s_cs[kMaxTok][kMaxPairs + 1];
-  __shared__ __attribute__((aligned(16))) float s_row[kThreads * 8];
-  __shared__ float s_red[BWD && NORM ? kThreads * 8 : 1];
-  const int tid = threadIdx.x, lane = tid % LPR, grp = tid / LPR;
-  const int c0 = lane * 8, hd = a.hd;
+// LDS of one wave: its writes are in order before its reads.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-  // partner channel and pair of each of this lane's channels; pass-through: pair npairs
-  // (cos 1, sin 0) and itself
-  int other[8], pair[8];
-  float sign[8];
+// Sum over the LPR lanes of a row, the same bits in each; `buf`: the row's floats in LDS.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, int sub, float* buf) {
+  if constexpr ((LPR & (LPR - 1)) == 0) {
+    return group_sum<LPR>(v);
+  } else {
+    buf[sub] = v;
+    wave_fence();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LPR; ++i) s += buf[i];
+    wave_fence();
+    return s;
+  }
+}
+
+// LPR: lanes of a row (8 channels each).
+template <typename T, int LPR, bool NORM, bool BWD, bool VEC, bool INTER>
+__global__ __launch_bounds__(kThreads, 4) void qk_rope_kernel(const RopeArgs a) {
+  constexpr int kRows = 64 / LPR;  // rows of a wave at a time (lanes behind them idle)
+  constexpr int kAhead = sizeof(T) == 2 && !(NORM && BWD) ? 2 : 1;  // rows of a lane in flight
+  constexpr bool kExchange = !INTER || (NORM && (LPR & (LPR - 1)) != 0);
+  constexpr bool kRowBuf = kExchange || (NORM && BWD);
+  __shared__ float2 s_cs[kWaves][kMaxPairs + 1];
+  __shared__ __attribute__((aligned(16))) float s_row[kRowBuf ? kThreads * 8 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int sub = lane % LPR, grp = lane / LPR;  // grp == kRows: an idle lane
+  const int c0 = sub * 8, hd = a.hd;
+
+  // of each of this lane's channels: its pair (pass-through: npairs, cos 1, sin 0), partner << 8
+  // and, at bit 16, whether the partner's term is subtracted
+  int code[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int c = c0 + e;
-    other[e] = c;
-    pair[e] = a.npairs;
-    sign[e] = 0.0f;
+    code[e] = a.npairs | (c << 8);
     int at = 0;
     for (int x = 0; x < a.n_axes; ++x) {
       const int d = a.axis[x], l = c - at;
       if (l >= 0 && l < d) {
         const int half = d / 2;
-        const bool second = a.interleaved ? (l & 1) : l >= half;
-        other[e] = a.interleaved ? (c ^ 1) : (second ? c - half : c + half);
         // axes are even and begin at even channels, so c ^ 1 is within the axis
-        pair[e] = at / 2 + (a.interleaved ? l / 2 : (second ? l - half : l));
-        sign[e] = second ? 1.0f : -1.0f;
+        const bool second = INTER ? (l & 1) : l >= half;
+        const int other = INTER ? (c ^ 1) : (second ? c - half : c + half);
+        const int pair = at / 2 + (INTER ? l / 2 : (second ? l - half : l));
+        code[e] = pair | (other << 8) | (second == BWD ? 1 << 16 : 0);  // backward: turns back
       }
       at += d;
     }
-    if (BWD) sign[e] = -sign[e];
   }
 
-  float w[2][8], dw[2][8];
+  const int which = blockIdx.z;  // 0: q, 1: k
+  const int heads = a.heads[which];
+  float w[8], dw[8];
   if (NORM) {
+    if (a.w[which] == nullptr) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (a.w[t] != nullptr) {
-        if (a.w_f32)
-          load8<float, false>(static_cast<const float*>(a.w[t]), c0, hd, w[t]);
-        else
-          load8<T, false>(static_cast<const T*>(a.w[t]), c0, hd, w[t]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[t][e] = 1.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dw[t][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+    } else if (a.w_f32) {
+      load_weight<float>(a.w[which], c0, hd, w);
+    } else {
+      load_weight<T>(a.w[which], c0, hd, w);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = 0.0f;
   }
 
-  float* const row = s_row + grp * LPR * 8;
-  const int nheads = a.heads[0] + a.heads[1];
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tok; t0 < a.tokens;
-       t0 += static_cast<int64_t>(gridDim.x) * a.tok) {
-    const int nt = static_cast<int>(a.tokens - t0 < a.tok ? a.tokens - t0 : a.tok);
-    __syncthreads();
-    for (int i = tid; i < nt * (a.npairs + 1); i += kThreads) {
-      const int t = i / (a.npairs + 1), p = i - t * (a.npairs + 1);
-      float2 cs = make_float2(1.0f, 0.0f);
-      if (p < a.npairs) {
-        int x = 0, end = a.axis[0] / 2;
-        while (p >= end) end += a.axis[++x] / 2;
-        const double r = position(a, (t0 + t) % a.pos_rows, x) * a.rev[p];
-        sincospif(2.0f * static_cast<float>(r - rint(r)), &cs.y, &cs.x);
-      }
-      s_cs[t][p] = cs;
+  float* const row = s_row + (kRowBuf ? (wave * 64 + grp * LPR) * 8 : 0);
+  if (lane == 0) s_cs[wave][a.npairs] = make_float2(1.0f, 0.0f);
+  const float inv_hd = 1.0f / hd;
+
+  // heads [h0, h1) are this workgroup's
+  const int per = (heads + gridDim.y - 1) / gridDim.y;
+  const int h0 = blockIdx.y * per, h1 = h0 + per < heads ? h0 + per : heads;
+  const T* const xs = static_cast<const T*>(a.x[which]);
+  const T* const dys = static_cast<const T*>(a.dy[which]);
+  T* const ys = static_cast<T*>(a.y[which]);
+  const int64_t stride = a.stride[which], out_stride = static_cast<int64_t>(heads) * hd;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWaves;
+
+  Raw<T> rx[kAhead], ry[kAhead];  // the next rows
+  const auto load = [&](int64_t tok, int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int hh = h + i * kRows + grp;
+      const bool live = hh < h1 && grp < kRows;
+      if (NORM || !BWD) rx[i].template load<VEC>(xs + tok * stride + hh * hd, c0, hd, live);
+      if (BWD) ry[i].template load<VEC>(dys + tok * out_stride + hh * hd, c0, hd, live);
     }
-    __syncthreads();
-    const int tasks = nt * nheads;
-    for (int task = grp; task < (tasks + kGroups - 1) / kGroups * kGroups; task += kGroups) {
-      const bool live = task < tasks;
-      const int t = live ? task / nheads : 0, hh = live ? task - t * nheads : 0;
-      const int which = hh >= a.heads[0];
-      const int h = which ? hh - a.heads[0] : hh;
-      const int64_t tok = t0 + t;
-      const int64_t out_at = (tok * a.heads[which] + h) * hd;
-      const T* xp = static_cast<const T*>(a.x[which]) + tok * a.stride[which] + int64_t(h) * hd;
-      float v[8], x[8], r = 1.0f;
-      if (live && (NORM || !BWD)) {
-        load8<T, VEC>(xp, c0, hd, x);
-      } else {
+  };
+  int64_t tok = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
+  if (tok < a.tokens) load(tok, h0);
+  for (; tok < a.tokens; tok += step) {
+    wave_fence();
+    const int64_t prow = a.pos_rows == a.tokens ? tok : tok % a.pos_rows;
+    for (int p = lane; p < a.npairs; p += 64) {
+      int x = 0, end = a.axis[0] / 2;
+      while (p >= end) end += a.axis[++x] / 2;
+      const double r = position(a, prow, x) * a.rev[p];
+      float2 cs;
+      sincospif(2.0f * static_cast<float>(r - rint(r)), &cs.y, &cs.x);
+      s_cs[wave][p] = cs;
+    }
+    wave_fence();
+    float cs[8], sn[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = s_cs[wave][code[e] & 255];
+      cs[e] = v.x;
+      sn[e] = code[e] & (1 << 16) ? -v.y : v.y;
+    }
+
+    for (int h = h0; h < h1; h += kAhead * kRows) {
+      Raw<T> cx[kAhead], cy[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        cx[i] = rx[i];
+        cy[i] = ry[i];
       }
-      if (BWD) {
-        if (live) {
-          load8<T, VEC>(static_cast<const T*>(a.dy[which]) + out_at, c0, hd, v);
+      if (h + kAhead * kRows < h1)
+        load(tok, h + kAhead * kRows);
+      else if (tok + step < a.tokens)
+        load(tok + step, h0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int hh = h + i * kRows + grp;
+        if (h + i * kRows >= h1) break;
+        float v[8], x[8], r = 1.0f;
+        if (NORM || !BWD) cx[i].get(x);
+        if (BWD) cy[i].get(v);
+        if (NORM) {
+          float ss = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+          ss = row_sum<LPR>(ss, sub, row);
+          r = rsqrtf(ss * inv_hd + a.eps);
+        }
+        if (!BWD) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = NORM ? x[e] * r * w[e] : x[e];
+        }
+        float o[8];
+        if (INTER) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = v[e ^ 1];
         } else {
+          *reinterpret_cast<float4*>(row + c0) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(row + c0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+          wave_fence();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+          for (int e = 0; e < 8; ++e) o[e] = row[(code[e] >> 8) & 255];
+          wave_fence();
         }
-      }
-      if (NORM) {
-        float ss = 0.0f;
+        float g[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-        ss = group_sum<LPR>(ss);
-        r = 1.0f / sqrtf(ss / hd + a.eps);
-      }
-      if (!BWD) {
+        for (int e = 0; e < 8; ++e) g[e] = v[e] * cs[e] + sn[e] * o[e];
+        if (a.pass) {
+          // channels that pass through are not multiplied by zero (they may be infinite)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = NORM ? x[e] * r * (which ? w[1][e] : w[0][e]) : x[e];
-      }
-      float o[8];
-      if (a.interleaved) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = v[e ^ 1];
-      } else {
-        // a row belongs to lanes of one wave: its writes and reads are in order
-        *reinterpret_cast<float4*>(row + c0) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(row + c0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = row[other[e]];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
-      float g[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 cs = s_cs[t][pair[e]];
-        // a pass-through channel is not multiplied by its partner's zero (it may be infinite)
-        g[e] = sign[e] == 0.0f ? v[e] : v[e] * cs.x + sign[e] * (o[e] * cs.y);
-      }
-      if (BWD && NORM) {
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float gx = g[e] * x[e];
-          const float we = which ? w[1][e] : w[0][e];
-          if (which) dw[1][e] += gx * r; else dw[0][e] += gx * r;
-          dot += gx * we;
+          for (int e = 0; e < 8; ++e) g[e] = (code[e] & 255) == a.npairs ? v[e] : g[e];
         }
-        dot = group_sum<LPR>(dot);
-        const float f = r * r * (r * (dot / hd));
+        if (BWD && NORM) {
+          float dot = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = r * (g[e] * (which ? w[1][e] : w[0][e])) - x[e] * f;
+          for (int e = 0; e < 8; ++e) {
+            dw[e] += g[e] * x[e] * r;
+            g[e] *= w[e];
+            dot += g[e] * x[e];
+          }
+          dot = row_sum<LPR>(dot, sub, row);
+          const float f = r * r * (r * (dot * inv_hd));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = r * g[e] - x[e] * f;
+        }
+        if (hh < h1 && grp < kRows)
+          store8<T, VEC>(ys + tok * out_stride + hh * hd, c0, hd, g);
       }
-      if (live) store8<T, VEC>(static_cast<T*>(a.y[which]) + out_at, c0, hd, g);
     }
   }
 
   if (BWD && NORM && a.dw != nullptr) {
+    __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s_red[grp * LPR * 8 + c0 + e] = dw[t][e];
-      __syncthreads();
-      for (int c = tid; c < hd; c += kThreads) {
-        float s = 0.0f;
-        for (int g = 0; g < kGroups; ++g) s += s_red[g * LPR * 8 + c];
-        a.dw[(static_cast<int64_t>(blockIdx.x) * 2 + t) * hd + c] = s;
-      }
+    for (int e = 0; e < 8; ++e) row[c0 + e] = dw[e];
+    __syncthreads();
+    for (int c = tid; c < hd; c += kThreads) {
+      float s = 0.0f;
+      for (int g = 0; g < kWaves * kRows; ++g)
+        s += s_row[(g / kRows * 64 + g % kRows * LPR) * 8 + c];
+      const int64_t blk = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+      a.dw[(blk * 2 + which) * hd + c] = s;
     }
   }
 }
 
 // Sum of the workgroups' partial weight gradients, in a fixed order: 16 columns a workgroup,
-// 16 threads a column.
+// 64 threads a column.
 template <typename T>
-__global__ __launch_bounds__(256) void dw_sum_kernel(const float* __restrict__ part, int blocks,
-                                                     int hd, T* dwq, T* dwk) {
-  __shared__ float red[16][17];
+__global__ __launch_bounds__(1024) void dw_sum_kernel(const float* __restrict__ part, int blocks,
+                                                      int hd, T* dwq, T* dwk) {
+  __shared__ float red[64][17];
   const int col = blockIdx.x * 16 + threadIdx.x % 16, r0 = threadIdx.x / 16;
   float s = 0.0f;
-  if (col < 2 * hd)
-    for (int b = r0; b < blocks; b += 16) s += part[static_cast<int64_t>(b) * 2 * hd + col];
+  if (col < 2 * hd) {
+#pragma unroll 4
+    for (int b = r0; b < blocks; b += 64) s += part[static_cast<int64_t>(b) * 2 * hd + col];
+  }
   red[r0][threadIdx.x % 16] = s;
   __syncthreads();
   if (r0 == 0 && col < 2 * hd) {
     s = 0.0f;
-    for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+    for (int i = 0; i < 64; ++i) s += red[i][threadIdx.x];
     T* const out = col < hd ? dwq : dwk;
     if (out != nullptr) out[col < hd ? col : col - hd] = from_f32<T>(s);
   }
 }
 
-int64_t blocks_of(const msd_qk_rope_desc& d, int tok, bool bwd) {
-  const int64_t n = (d.tokens + tok - 1) / tok;
-  const int64_t cap = bwd ? kBwdBlocks : int64_t(1) << 20;
-  return n < cap ? n : cap;
+// Lanes of a head's row: 10 and 12 (head sizes to 80 and 96) leave 4 of 64 lanes idle where 16
+// would leave 24 and 16.
+int lanes_of(int hd) {
+  for (int n : {4, 8, 10, 12, 16})
+    if (hd <= 8 * n) return n;
+  return 32;
 }
 
-// Tokens of a workgroup's step: as many as share their angles' cost, fewer where that would
-// leave compute units idle (256 of them, a few workgroups each).
-int tokens_of_step(const msd_qk_rope_desc& d) {
-  int tok = kMaxTok;
-  while (tok > 1 && d.tokens < int64_t(tok) * 1024) tok /= 2;
-  return tok;
+struct Shape {
+  int64_t x;  // workgroups along the tokens
+  int y;      // and along the heads
+};
+
+// One token a wave; where that is under 2,048 waves (eight a compute unit), the heads are split
+// too, down to one row of a lane group each.
+Shape grid_of(const msd_qk_rope_desc& d, bool bwd) {
+  const int rows = 64 / lanes_of(d.head_dim);
+  const int steps = (d.q_heads + rows - 1) / rows;
+  Shape s{(d.tokens + kWaves - 1) / kWaves, 1};
+  while (s.y * 2 <= steps && d.tokens * s.y < 2048) s.y *= 2;
+  const int64_t cap = bwd && d.norm ? kMaxBwdBlocks : kMaxBlocks;
+  if (s.x > cap) s.x = cap;
+  return s;
 }
 
 template <typename T, int LPR, bool NORM, bool BWD>
-void launch_vec(const RopeArgs& a, unsigned blocks, bool vec, hipStream_t s) {
-  if (vec)
-    qk_rope_kernel<T, LPR, NORM, BWD, true><<<blocks, kThreads, 0, s>>>(a);
-  else
-    qk_rope_kernel<T, LPR, NORM, BWD, false><<<blocks, kThreads, 0, s>>>(a);
+void launch_vec(const RopeArgs& a, Shape g, bool vec, bool inter, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(g.x), g.y, a.heads[1] > 0 ? 2 : 1);
+  if (vec && inter) qk_rope_kernel<T, LPR, NORM, BWD, true, true><<<grid, kThreads, 0, s>>>(a);
+  else if (vec) qk_rope_kernel<T, LPR, NORM, BWD, true, false><<<grid, kThreads, 0, s>>>(a);
+  else if (inter) qk_rope_kernel<T, LPR, NORM, BWD, false, true><<<grid, kThreads, 0, s>>>(a);
+  else qk_rope_kernel<T, LPR, NORM, BWD, false, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <typename T, int LPR>
-void launch_kind(const RopeArgs& a, unsigned blocks, bool norm, bool bwd, bool vec,
+void launch_kind(const RopeArgs& a, Shape g, bool norm, bool bwd, bool vec, bool inter,
                  hipStream_t s) {
-  if (norm && bwd) launch_vec<T, LPR, true, true>(a, blocks, vec, s);
-  else if (norm) launch_vec<T, LPR, true, false>(a, blocks, vec, s);
-  else if (bwd) launch_vec<T, LPR, false, true>(a, blocks, vec, s);
-  else launch_vec<T, LPR, false, false>(a, blocks, vec, s);
+  if (norm && bwd) launch_vec<T, LPR, true, true>(a, g, vec, inter, s);
+  else if (norm) launch_vec<T, LPR, true, false>(a, g, vec, inter, s);
+  else if (bwd) launch_vec<T, LPR, false, true>(a, g, vec, inter, s);
+  else launch_vec<T, LPR, false, false>(a, g, vec, inter, s);
 }
 
 template <typename T>
-void launch_type(const RopeArgs& a, unsigned blocks, bool norm, bool bwd, bool vec,
+void launch_type(const RopeArgs& a, Shape g, bool norm, bool bwd, bool vec, bool inter,
                  hipStream_t s) {
-  if (a.hd <= 32) launch_kind<T, 4>(a, blocks, norm, bwd, vec, s);
-  else if (a.hd <= 64) launch_kind<T, 8>(a, blocks, norm, bwd, vec, s);
-  else if (a.hd <= 128) launch_kind<T, 16>(a, blocks, norm, bwd, vec, s);
-  else launch_kind<T, 32>(a, blocks, norm, bwd, vec, s);
+  switch (lanes_of(a.hd)) {
+    case 4: return launch_kind<T, 4>(a, g, norm, bwd, vec, inter, s);
+    case 8: return launch_kind<T, 8>(a, g, norm, bwd, vec, inter, s);
+    case 10: return launch_kind<T, 10>(a, g, norm, bwd, vec, inter, s);
+    case 12: return launch_kind<T, 12>(a, g, norm, bwd, vec, inter, s);
+    case 16: return launch_kind<T, 16>(a, g, norm, bwd, vec, inter, s);
+    default: return launch_kind<T, 32>(a, g, norm, bwd, vec, inter, s);
+  }
 }
 
 }  // namespace
 
 size_t qk_rope_bwd_ws_bytes(const msd_qk_rope_desc& d) {
   if (!d.norm) return 0;
-  return static_cast<size_t>(blocks_of(d, tokens_of_step(d), true)) * 2 * d.head_dim * sizeof(float);
+  const Shape g = grid_of(d, true);
+  return static_cast<size_t>(g.x) * g.y * 2 * d.head_dim * sizeof(float);
 }
 
 hipError_t launch_qk_rope(const msd_qk_rope_desc& d, const QkRopePtrs& p, bool bwd, void* ws,
@@ -360,17 +449,18 @@ hipError_t launch_qk_rope(const msd_qk_rope_desc& d, const QkRopePtrs& p, bool b
   a.dw = static_cast<float*>(ws);
   a.hd = d.head_dim;
   a.n_axes = d.n_axes;
-  a.interleaved = d.interleaved;
   a.pos_dtype = d.pos_dtype;
   a.w_f32 = d.weight_dtype == MSD_F32;
   a.eps = d.eps;
   for (int x = 0; x < 3; ++x) a.grid[x] = d.grid[x];
-  a.tok = tokens_of_step(d);
   for (int x = 0; x < d.n_axes; ++x) {
+    // theta^(-2 i / d) by products in extended precision: a few steps of 2^-64 off
+    const long double step = powl(static_cast<long double>(d.theta), -2.0L / d.axis_dims[x]);
+    long double f = 1.0L / 6.283185307179586476925287L;
     a.axis[x] = d.axis_dims[x];
-    for (int i = 0; i < d.axis_dims[x] / 2; ++i)
-      a.rev[a.npairs++] = std::pow(d.theta, -2.0 * i / d.axis_dims[x]) / 6.283185307179586476925;
+    for (int i = 0; i < d.axis_dims[x] / 2; ++i, f *= step) a.rev[a.npairs++] = static_cast<double>(f);
   }
+  a.pass = 2 * a.npairs < d.head_dim;
   const size_t e = d.dtype == MSD_BF16 ? 2 : 4;
   bool vec = d.head_dim % 8 == 0;
   for (int t = 0; t < 2; ++t) {
@@ -379,21 +469,23 @@ hipError_t launch_qk_rope(const msd_qk_rope_desc& d, const QkRopePtrs& p, bool b
     for (const void* ptr : {a.x[t], a.dy[t], static_cast<const void*>(a.y[t])})
       vec = vec && reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
   }
-  const unsigned blocks = static_cast<unsigned>(blocks_of(d, a.tok, bwd));
-  if (blocks > 0 && d.dtype == MSD_BF16)
-    launch_type<bf16>(a, blocks, d.norm != 0, bwd, vec, s);
-  else if (blocks > 0)
-    launch_type<float>(a, blocks, d.norm != 0, bwd, vec, s);
+  const Shape g = grid_of(d, bwd);
+  if (g.x > 0 && d.dtype == MSD_BF16)
+    launch_type<bf16>(a, g, d.norm != 0, bwd, vec, d.interleaved != 0, s);
+  else if (g.x > 0)
+    launch_type<float>(a, g, d.norm != 0, bwd, vec, d.interleaved != 0, s);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || !bwd || !d.norm) return err;
   const unsigned cols = static_cast<unsigned>((2 * d.head_dim + 15) / 16);
+  const int blocks = static_cast<int>(g.x * g.y);
   if (a.w_f32)
-    dw_sum_kernel<float><<<cols, 256, 0, s>>>(a.dw, blocks, d.head_dim,
-                                              static_cast<float*>(p.dw[0]),
-                                              static_cast<float*>(p.dw[1]));
+    dw_sum_kernel<float><<<cols, 1024, 0, s>>>(a.dw, blocks, d.head_dim,
+                                               static_cast<float*>(p.dw[0]),
+                                               static_cast<float*>(p.dw[1]));
   else
-    dw_sum_kernel<bf16><<<cols, 256, 0, s>>>(a.dw, blocks, d.head_dim, static_cast<bf16*>(p.dw[0]),
-                                             static_cast<bf16*>(p.dw[1]));
+    dw_sum_kernel<bf16><<<cols, 1024, 0, s>>>(a.dw, blocks, d.head_dim,
+                                              static_cast<bf16*>(p.dw[0]),
+                                              static_cast<bf16*>(p.dw[1]));
   return hipGetLastError();
 }
 
