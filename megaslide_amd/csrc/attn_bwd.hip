@@ -21,20 +21,21 @@ constexpr int kNT = kNW * 64;
 constexpr int kTile = kNW * 32;  // stationary rows of a workgroup
 constexpr int kBN = 64;          // keys of a passing tile (dQ)
 constexpr int kBQ = 64;          // rows of a passing tile (dK, dV)
+constexpr int kEnoughWgs = 1024;
 
 template <typename T, int HD, bool VEC>
-__global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
+__global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_bwd_dq_kernel(
     const AttnArgs a, const T* __restrict__ out, const T* __restrict__ dout,
     const float* __restrict__ lse, const float* __restrict__ dlse, T* __restrict__ dq,
-    float2* __restrict__ stats, int64_t slots) {
+    float2* __restrict__ stats, float* __restrict__ part, int nsplit, int slots) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kKK = HD / 16, kBlk = HD / 32;
   __shared__ __attribute__((aligned(16))) T s_k[2][kBN * HD];
   __shared__ __attribute__((aligned(16))) T s_v[sizeof(T) == 2 ? 2 : 1][kBN * HD];
 
-  int64_t id = blockIdx.x;
-  const int kvh = static_cast<int>(id % a.hk);
-  id /= a.hk;
+  const int hs = blockIdx.x / static_cast<unsigned>(a.hk);
+  const int kvh = blockIdx.x - hs * a.hk;
+  const int id = hs / nsplit, split = hs - id * nsplit;
   const Span sp = find_span(a, a.cu_q == nullptr ? id : slots - 1 - id, a.group, kTile, false);
   if (sp.tile < 0) return;
 
@@ -44,12 +45,12 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
   const bool mine = row0 + (lane & 31) < rows;
   const int row = mine ? row0 + (lane & 31) : rows - 1;
   const int tok = row / a.group, head = kvh * a.group + row % a.group;
-  int limit = sp.lk, low = sp.lk, top = sp.lk, end = sp.lk;
+  int limit = sp.lk, all = sp.lk, top = sp.lk, end = sp.lk;
   if (a.causal) {
     const int last = (sp.tile + 1) * kTile < rows ? (sp.tile + 1) * kTile : rows;
     const int wlast = row0 + 32 < rows ? row0 + 32 : rows;
     limit = tok + 1 + shift;
-    low = (row0 < rows ? row0 : rows - 1) / a.group + 1 + shift;
+    all = sp.tile * kTile / a.group + 1 + shift;
     top = (wlast - 1) / a.group + 1 + shift;
     end = (last - 1) / a.group + 1 + shift;
     end = end > 0 ? end : 0;
@@ -73,14 +74,15 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
   if (dlse != nullptr) delta -= dlse[at_row];
   float ls = lse[at_row];
   ls = ls == -INFINITY ? INFINITY : ls * kLog2e;  // a row without keys has no weights
-  if (mine && g == 0) stats[at_row] = make_float2(ls, delta);
+  if (mine && g == 0 && split == 0) stats[at_row] = make_float2(ls, delta);
 
   f32x16 acc[kBlk];
 #pragma unroll
   for (int b = 0; b < kBlk; ++b) acc[b] = f32x16{};
   const float c = a.scale * kLog2e;
 
-  const int stop = (end + kBN - 1) / kBN;
+  int first, stop;
+  split_range((end + kBN - 1) / kBN, nsplit, split, &first, &stop);
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.ks + int64_t(kvh) * a.hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
   constexpr bool kTwo = sizeof(T) == 2;  // V double-buffered too (fp32: LDS holds three tiles)
@@ -92,21 +94,22 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
     tk.load([&](int r) { return kt + r * a.ks; }, n, a.hd);
     tv.load([&](int r) { return vt + r * a.vs; }, n, a.hd);
   };
-  if (stop > 0) {
-    load(0);
+  if (first < stop) {
+    load(first);
     tk.store(s_k[0]);
     tv.store(s_v[0]);
   }
   __syncthreads();
 
-  for (int t = 0; t < stop; ++t) {
-    const int buf = t & 1, vbuf = kTwo ? buf : 0, k0 = t * kBN;
+  Finite<T> fin;
+  const auto step = [&](int t, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked_c)::value;
+    const int buf = (t - first) & 1, vbuf = kTwo ? buf : 0, k0 = t * kBN;
     const bool more = t + 1 < stop;
     if (more) load(t + 1);
-    if (row0 < rows && k0 < top) {
+    if (row0 < rows && (!kMasked || k0 < top)) {
 #pragma unroll
       for (int b = 0; b < kBN / 32; ++b) {
-        const int kb = k0 + b * 32;
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int i = 0; i < kKK; ++i) {
@@ -114,23 +117,9 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
           dp = mma(row_frag<T, HD>(s_v[vbuf], b * 32 + (lane & 31), i * 16 + g * 8), go[i], dp);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
+        for (int r = 0; r < 16; ++r) {
           s[r] = __builtin_amdgcn_exp2f(s[r] * c - ls) * (dp[r] - delta);
-        const bool masked = kb + 32 > low;
-        bool bad = false;
-        if (masked) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (kb + 8 * (r / 4) + 4 * g + r % 4 >= limit) s[r] = 0.0f;
-          if (a.causal) {
-            // keys that are not finite make the weights of rows that see them NaN; the others
-            // must not meet them
-#pragma unroll
-            for (int d = 0; d < kBlk; ++d)
-              bad |= nonfinite(col_frag<T, HD>(s_k[buf], b * 32, d)) ||
-                     nonfinite(col_frag<T, HD>(s_k[buf], b * 32 + 16, d));
-            bad = __any(bad);
-          }
+          if (kMasked && k0 + b * 32 + 8 * (r / 4) + 4 * g + r % 4 >= limit) s[r] = 0.0f;
         }
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -138,7 +127,8 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
 #pragma unroll
           for (int d = 0; d < kBlk; ++d) {
             Frag kf = col_frag<T, HD>(s_k[buf], b * 32 + t2 * 16, d);
-            if (bad) kf = finite_part(kf);
+            // (a row that sees a key that is not finite has weights that are NaN)
+            if (kMasked) kf = fin(kf);
             acc[d] = mma(kf, ds, acc[d]);
           }
         }
@@ -150,16 +140,26 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dq_kernel(
       tv.store(s_v[kTwo ? buf ^ 1 : 0]);
     }
     __syncthreads();
-  }
+  };
+  int t = first, whole = all > 0 ? all / kBN : 0;  // tiles that every row sees whole
+  whole = whole < stop ? whole : stop;
+  for (; t < whole; ++t) step(t, std::false_type{});
+  for (; t < stop; ++t) step(t, std::true_type{});
   if (!mine) return;
+  float* const po = part + (split * a.total_q * a.hq + at_row) * HD;
 #pragma unroll
-  for (int d = 0; d < kBlk; ++d) store_block<T, VEC>(dq + at_row * a.hd, acc[d], d, a.scale, a.hd);
+  for (int d = 0; d < kBlk; ++d) {
+    if (nsplit > 1)
+      store_block<float, true>(po, acc[d], d, a.scale, HD);
+    else
+      store_block<T, VEC>(dq + at_row * a.hd, acc[d], d, a.scale, a.hd);
+  }
 }
 
 template <typename T, int HD, bool VEC>
-__global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
+__global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_bwd_dkv_kernel(
     const AttnArgs a, const T* __restrict__ dout, const float2* __restrict__ stats,
-    T* __restrict__ dk, T* __restrict__ dv, int64_t slots) {
+    T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kKK = HD / 16, kBlk = HD / 32;
   constexpr int kBufs = sizeof(T) == 2 ? 2 : 1;
@@ -168,10 +168,11 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
   __shared__ __attribute__((aligned(16))) float s_lse[kBufs][kBQ];
   __shared__ __attribute__((aligned(16))) float s_delta[kBufs][kBQ];
 
-  int64_t id = blockIdx.x;
-  const int kvh = static_cast<int>(id % a.hk);
-  id /= a.hk;
-  const Span sp = find_span(a, a.cu_k == nullptr ? id : slots - 1 - id, 1, kTile, true);
+  // first tiles first: causal ones have the most rows
+  const int hs = blockIdx.x / static_cast<unsigned>(a.hk);
+  const int kvh = blockIdx.x - hs * a.hk;
+  const int id = hs / nsplit, split = hs - id * nsplit;
+  const Span sp = find_span(a, id, 1, kTile, true);
   if (sp.tile < 0) return;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5;
@@ -179,10 +180,9 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
   const int key0 = sp.tile * kTile + wave * 32;
   const bool mine = key0 + (lane & 31) < sp.lk;
   const int key = mine ? key0 + (lane & 31) : sp.lk - 1;
-  const int wlast = key0 + 31 < sp.lk ? key0 + 31 : sp.lk - 1;  // the wave's last key
   // rows from `first` on see this lane's key, from `wfirst` on some key of the wave, from
-  // `wall` on all of them
-  int first = 0, wfirst = 0, wall = 0, begin = 0;
+  // `begin` on some key of the workgroup, from `all` on all of them
+  int first = 0, wfirst = 0, all = 0, begin = 0;
   if (a.causal) {
     const auto from = [&](int k) {
       const int64_t i = static_cast<int64_t>(k) - shift;
@@ -190,7 +190,8 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
     };
     first = from(key);
     wfirst = from(key0 < sp.lk ? key0 : sp.lk - 1);
-    wall = from(wlast);
+    const int last = (sp.tile + 1) * kTile - 1;
+    all = from(last < sp.lk ? last : sp.lk - 1);
     begin = from(sp.tile * kTile);
   }
 
@@ -234,14 +235,19 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
       s_delta[buf][tid] = st.y;
     }
   };
-  const int t0 = begin / kBQ, stop = (rows + kBQ - 1) / kBQ;
+  int t0, stop;
+  split_range((rows + kBQ - 1) / kBQ - begin / kBQ, nsplit, split, &t0, &stop);
+  t0 += begin / kBQ;
+  stop += begin / kBQ;
   if (t0 < stop) {
     load(t0);
     store(0);
   }
   __syncthreads();
 
-  for (int t = t0; t < stop; ++t) {
+  Finite<T> finq, fing;
+  const auto step = [&](int t, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked_c)::value;
     const int buf = kBufs == 2 ? (t - t0) & 1 : 0;
     const bool more = t + 1 < stop;
     if (more) load(t + 1);
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
 #pragma unroll
       for (int b = 0; b < kBQ / 32; ++b) {
         const int r0 = t * kBQ + b * 32;
-        if (r0 + 32 <= wfirst || r0 >= rows) continue;
+        if (kMasked && r0 + 32 <= wfirst) continue;
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int i = 0; i < kKK; ++i) {
@@ -266,21 +272,8 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
             const int r = 4 * i + j;
             p[r] = __builtin_amdgcn_exp2f(s[r] * c - ls[j]);
             s[r] = p[r] * (dp[r] - de[j]);
+            if (kMasked && r0 + 8 * i + 4 * g + j < first) p[r] = s[r] = 0.0f;
           }
-        }
-        const auto seen = [&](int r) { return r0 + 8 * (r / 4) + 4 * g + r % 4 >= first; };
-        bool bad = false;
-        if (r0 < wall) {  // causal only
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!seen(r)) p[r] = s[r] = 0.0f;
-#pragma unroll
-          for (int d = 0; d < kBlk; ++d)
-            bad |= nonfinite(col_frag<T, HD>(s_q[buf], b * 32, d)) ||
-                   nonfinite(col_frag<T, HD>(s_q[buf], b * 32 + 16, d)) ||
-                   nonfinite(col_frag<T, HD>(s_g[buf], b * 32, d)) ||
-                   nonfinite(col_frag<T, HD>(s_g[buf], b * 32 + 16, d));
-          bad = __any(bad);
         }
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -289,34 +282,65 @@ __global__ __launch_bounds__(kNT, 1) void attn_bwd_dkv_kernel(
           for (int d = 0; d < kBlk; ++d) {
             Frag gf = col_frag<T, HD>(s_g[buf], b * 32 + t2 * 16, d);
             Frag qf = col_frag<T, HD>(s_q[buf], b * 32 + t2 * 16, d);
-            if (bad) {
-              gf = finite_part(gf);
-              qf = finite_part(qf);
+            if (kMasked) {
+              gf = fing(gf);
+              qf = finq(qf);  // (a query that is not finite makes the weights it has NaN)
             }
             av[d] = mma(gf, pf, av[d]);
             ak[d] = mma(qf, df, ak[d]);
           }
-        }
-        if (bad) {
-#pragma unroll
-          for (int d = 0; d < kBlk; ++d)
-            add_nonfinite<T>(av[d], p, seen, [&](int t2) {
-              return col_frag<T, HD>(s_g[buf], b * 32 + t2 * 16, d);
-            });
         }
       }
     }
     if (kBufs == 1) __syncthreads();
     if (more) store(kBufs == 2 ? buf ^ 1 : 0);
     __syncthreads();
-  }
+  };
+  int t = t0, cut = (all + kBQ - 1) / kBQ;  // tiles from `cut` on see every key
+  cut = cut < t0 ? t0 : cut < stop ? cut : stop;
+  for (; t < cut; ++t) step(t, std::true_type{});
+  for (; t < stop; ++t) step(t, std::false_type{});
+  if (__any(fing.bad()))
+    add_nonfinite<T>(
+        av, t0 * kBQ, cut * kBQ < rows ? cut * kBQ : rows, a.hd,
+        [=](int r) {
+          const int tok = r / a.group;
+          return dout + ((sp.q0 + tok) * a.hq + kvh * a.group + (r - tok * a.group)) * a.hd;
+        },
+        [=](int r) { return r >= first; });
   if (!mine) return;
-  const int64_t at_row = ((sp.k0 + key) * a.hk + kvh) * a.hd;
+  const int64_t at_row = (sp.k0 + key) * a.hk + kvh, n = a.total_k * a.hk;
+  float* const po = part + (split * n + at_row) * HD;
 #pragma unroll
   for (int d = 0; d < kBlk; ++d) {
-    store_block<T, VEC>(dk + at_row, ak[d], d, a.scale, a.hd);
-    store_block<T, VEC>(dv + at_row, av[d], d, 1.0f, a.hd);
+    if (nsplit > 1) {
+      store_block<float, true>(po, ak[d], d, a.scale, HD);
+      store_block<float, true>(po + nsplit * n * HD, av[d], d, 1.0f, HD);
+    } else {
+      store_block<T, VEC>(dk + at_row * a.hd, ak[d], d, a.scale, a.hd);
+      store_block<T, VEC>(dv + at_row * a.hd, av[d], d, 1.0f, a.hd);
+    }
   }
+}
+
+// Adds the parts of gradients whose sums were split, in order: rows of HD floats to rows of hd
+// values; blockIdx.y: which of two (dk, dv).
+template <typename T>
+__global__ __launch_bounds__(256) void attn_add_kernel(const float* __restrict__ part, int nsplit,
+                                                       int64_t rows, int hd, int padded, T* out0,
+                                                       T* out1) {
+  const int quads = padded / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = i / quads;
+  const int c = static_cast<int>(i - row * quads) * 4;
+  if (row >= rows || c >= hd) return;
+  const float* p = part + (blockIdx.y * nsplit * rows + row) * padded + c;
+  f32x4 s = *reinterpret_cast<const f32x4*>(p);
+  for (int k = 1; k < nsplit; ++k) s += *reinterpret_cast<const f32x4*>(p + k * rows * padded);
+  T* const o = (blockIdx.y ? out1 : out0) + row * hd + c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < hd) o[j] = from_f32<T>(s[j]);
 }
 
 int64_t slots_of(int64_t total, int seqs, int64_t mul, bool packed) {
@@ -324,42 +348,101 @@ int64_t slots_of(int64_t total, int seqs, int64_t mul, bool packed) {
   return (total / seqs * mul + kTile - 1) / kTile * seqs;
 }
 
+// Workgroups along the other side's rows where the tiles alone leave compute units idle, or end
+// late with the longest sequence's tiles: `wgs` workgroups, a mean of `passing` tiles to pass.
+int splits(int64_t wgs, int64_t passing) {
+  if (wgs == 0 || wgs >= kEnoughWgs) return 1;
+  int64_t n = (kEnoughWgs + wgs - 1) / wgs;
+  const int64_t most = (passing + 3) / 4;  // four tiles each at least
+  n = n < most ? n : most;
+  return static_cast<int>(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+
+struct Plan {
+  int64_t q_slots, k_slots;
+  int q_split, k_split;
+};
+
+Plan plan(const msd_attn_desc& d, bool packed) {
+  const int group = d.num_heads / d.num_kv_heads;
+  Plan p;
+  p.q_slots = d.total_q > 0 ? slots_of(d.total_q, d.num_seqs, group, packed) : 0;
+  p.k_slots = d.total_k > 0 ? slots_of(d.total_k, d.num_seqs, 1, packed) : 0;
+  const int64_t keys = d.total_k / d.num_seqs / kBN, rows = d.total_q / d.num_seqs * group / kBQ;
+  p.q_split = splits(p.q_slots * d.num_kv_heads, keys);
+  p.k_split = splits(p.k_slots * d.num_kv_heads, rows);
+  return p;
+}
+
+int padded_hd(int hd) { return (hd + 31) / 32 * 32; }
+
+size_t part_bytes(const msd_attn_desc& d, bool packed) {
+  const Plan p = plan(d, packed);
+  const int64_t q = p.q_split > 1 ? p.q_split * d.total_q * d.num_heads : 0;
+  const int64_t k = p.k_split > 1 ? 2 * p.k_split * d.total_k * d.num_kv_heads : 0;
+  return static_cast<size_t>(q > k ? q : k) * padded_hd(d.head_dim) * sizeof(float);
+}
+
+size_t stats_bytes(const msd_attn_desc& d) {
+  return (static_cast<size_t>(d.total_q) * d.num_heads * sizeof(float2) + 255) / 256 * 256;
+}
+
 template <typename T, int HD, bool VEC>
-hipError_t launch_hd(const AttnArgs& a, const AttnBwdPtrs& p, float2* stats, hipStream_t s) {
-  const bool packed = a.cu_q != nullptr;
+hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p, void* ws,
+                     hipStream_t s) {
+  const Plan pl = plan(d, a.cu_q != nullptr);
   const T* dout = static_cast<const T*>(p.dout);
-  int64_t slots = slots_of(a.total_q, a.seqs, a.group, packed);
-  if (a.total_q > 0 && slots > 0)
-    attn_bwd_dq_kernel<T, HD, VEC><<<static_cast<unsigned>(slots * a.hk), kNT, 0, s>>>(
-        a, static_cast<const T*>(p.out), dout, p.lse, p.dlse, static_cast<T*>(p.dq), stats, slots);
+  T* const dq = static_cast<T*>(p.dq);
+  T* const dk = static_cast<T*>(p.dk);
+  T* const dv = static_cast<T*>(p.dv);
+  float2* const stats = static_cast<float2*>(ws);
+  // dq's parts are added up before dk's and dv's take their place
+  float* const part = reinterpret_cast<float*>(static_cast<char*>(ws) + stats_bytes(d));
+  const auto add = [&](int n, int64_t rows, T* o0, T* o1) {
+    attn_add_kernel<T><<<dim3(static_cast<unsigned>((rows * (HD / 4) + 255) / 256), o1 ? 2 : 1),
+                         256, 0, s>>>(part, n, rows, a.hd, HD, o0, o1);
+  };
+  if (pl.q_slots > 0) {
+    attn_bwd_dq_kernel<T, HD, VEC>
+        <<<static_cast<unsigned>(pl.q_slots * pl.q_split * a.hk), kNT, 0, s>>>(
+            a, static_cast<const T*>(p.out), dout, p.lse, p.dlse, dq, stats, part, pl.q_split,
+            static_cast<int>(pl.q_slots));
+    if (pl.q_split > 1) add(pl.q_split, a.total_q * a.hq, dq, nullptr);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  slots = slots_of(a.total_k, a.seqs, 1, packed);
-  if (a.total_k > 0 && slots > 0)
-    attn_bwd_dkv_kernel<T, HD, VEC><<<static_cast<unsigned>(slots * a.hk), kNT, 0, s>>>(
-        a, dout, stats, static_cast<T*>(p.dk), static_cast<T*>(p.dv), slots);
+  if (pl.k_slots > 0) {
+    attn_bwd_dkv_kernel<T, HD, VEC>
+        <<<static_cast<unsigned>(pl.k_slots * pl.k_split * a.hk), kNT, 0, s>>>(
+            a, dout, stats, dk, dv, part, pl.k_split);
+    if (pl.k_split > 1) add(pl.k_split, a.total_k * a.hk, dk, dv);
+  }
   return hipGetLastError();
 }
 
 template <typename T, int HD>
-hipError_t launch_vec(const AttnArgs& a, const AttnBwdPtrs& p, float2* st, bool vec,
-                      hipStream_t s) {
-  return vec ? launch_hd<T, HD, true>(a, p, st, s) : launch_hd<T, HD, false>(a, p, st, s);
+hipError_t launch_vec(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p, void* ws,
+                      bool vec, hipStream_t s) {
+  return vec ? launch_hd<T, HD, true>(d, a, p, ws, s) : launch_hd<T, HD, false>(d, a, p, ws, s);
 }
 
 template <typename T>
-hipError_t launch_type(const AttnArgs& a, const AttnBwdPtrs& p, float2* st, bool vec,
-                       hipStream_t s) {
-  if (a.hd <= 32) return launch_vec<T, 32>(a, p, st, vec, s);
-  if (a.hd <= 64) return launch_vec<T, 64>(a, p, st, vec, s);
-  if (a.hd <= 96) return launch_vec<T, 96>(a, p, st, vec, s);
-  return launch_vec<T, 128>(a, p, st, vec, s);
+hipError_t launch_type(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p, void* ws,
+                       bool vec, hipStream_t s) {
+  switch (padded_hd(a.hd)) {
+    case 32: return launch_vec<T, 32>(d, a, p, ws, vec, s);
+    case 64: return launch_vec<T, 64>(d, a, p, ws, vec, s);
+    case 96: return launch_vec<T, 96>(d, a, p, ws, vec, s);
+    default: return launch_vec<T, 128>(d, a, p, ws, vec, s);
+  }
 }
 
 }  // namespace
 
+// Upper bound over both forms (packed or equal lengths): the descriptor does not say which.
 size_t attn_bwd_ws_bytes(const msd_attn_desc& d) {
-  return static_cast<size_t>(d.total_q) * d.num_heads * sizeof(float2);
+  const size_t x = part_bytes(d, true), y = part_bytes(d, false);
+  return stats_bytes(d) + (x > y ? x : y);
 }
 
 hipError_t launch_attn_bwd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p,
@@ -368,9 +451,8 @@ hipError_t launch_attn_bwd(const msd_attn_desc& d, const AttnArgs& a, const Attn
   for (const void* ptr : {p.out, p.dout, static_cast<const void*>(p.dq),
                           static_cast<const void*>(p.dk), static_cast<const void*>(p.dv)})
     vec = vec && reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
-  float2* const st = static_cast<float2*>(ws);
-  return d.dtype == MSD_BF16 ? launch_type<bf16>(a, p, st, vec, s)
-                             : launch_type<float>(a, p, st, vec, s);
+  return d.dtype == MSD_BF16 ? launch_type<bf16>(d, a, p, ws, vec, s)
+                             : launch_type<float>(d, a, p, ws, vec, s);
 }
 
 }  // namespace msd

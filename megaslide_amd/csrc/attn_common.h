@@ -14,6 +14,8 @@
 #include "attn.h"
 #include "common.h"
 
+#include <type_traits>
+
 namespace msd {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -76,33 +78,47 @@ __device__ __forceinline__ F zero_frag() {
   return r;
 }
 
-// Whether a fragment holds an infinity or NaN.
-__device__ __forceinline__ bool nonfinite(const bf16x8& f) {
-  const u32x4 u = __builtin_bit_cast(u32x4, f);
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
-  return bad;
-}
-__device__ __forceinline__ bool nonfinite(const f32x8& f) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= (__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u;
-  return bad;
-}
+// Which places are masked is decided by comparing indexes, never by adding a large number, so a
+// masked score may be NaN.  In the products over rows (P V and those of the gradients) a masked
+// place has weight zero, but zero times an infinity or NaN is NaN: tiles that a causal mask cuts
+// enter those products by their finite part, and what was left out is noted in `seen_bad`
+// (nonzero) and added afterwards where it is seen.
+struct FiniteBf16 {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 ok = {1, 1, 1, 1, 1, 1, 1, 1};
 
-// The fragment with infinities and NaN as zeros.
-template <typename F>
-__device__ __forceinline__ F finite_part(const F& f) {
-  F r = f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x = static_cast<float>(f[j]);
-    if (!(fabsf(x) < INFINITY)) r[j] = 0;
+  __device__ __forceinline__ bf16x8 operator()(const bf16x8& f) {
+    const u16x8 u = __builtin_bit_cast(u16x8, f);
+    // 1 where the exponent is not all ones
+    const u16x8 lim = 0x7f80, one = 1;
+    const u16x8 fin = __builtin_elementwise_min(
+        __builtin_elementwise_sub_sat(lim, static_cast<u16x8>(u & static_cast<uint16_t>(0x7fff))),
+        one);
+    ok &= fin;
+    return __builtin_bit_cast(bf16x8, static_cast<u16x8>(u * fin));
   }
-  return r;
-}
+  __device__ __forceinline__ bool bad() const {
+    const u32x4 u = __builtin_bit_cast(u32x4, ok);
+    return (u[0] & u[1] & u[2] & u[3]) != 0x00010001u;
+  }
+};
+struct FiniteF32 {
+  bool any = false;
+
+  __device__ __forceinline__ f32x8 operator()(const f32x8& f) {
+    f32x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool fin = fabsf(f[j]) < INFINITY;
+      any |= !fin;
+      r[j] = fin ? f[j] : 0.0f;
+    }
+    return r;
+  }
+  __device__ __forceinline__ bool bad() const { return any; }
+};
+template <typename T>
+using Finite = std::conditional_t<sizeof(T) == 2, FiniteBf16, FiniteF32>;
 
 // Maximum and sum of a value over the two halves of a wave (lanes l and l ^ 32).
 __device__ __forceinline__ float half_max(float v) {
@@ -138,17 +154,18 @@ __device__ __forceinline__ int64_t bound_of(const int32_t* cu, int s, int64_t to
 // lengths stay on the device.  Rows behind the last sequence make one more sequence without a
 // counterpart.  Offsets that are not in order or out of range give wrong rows, never rows
 // outside the tensors.  `keys`: tiles of keys, else of queries.
-__device__ __forceinline__ Span find_span(const AttnArgs& a, int64_t slot, int mul, int tile,
+__device__ __forceinline__ Span find_span(const AttnArgs& a, int slot, int mul, int tile,
                                           bool keys) {
   Span r;
   const int32_t* cu = keys ? a.cu_k : a.cu_q;
   int s;
   if (cu == nullptr) {
-    // equal lengths: the last tiles of all sequences first (the longest ones when causal)
+    // equal lengths: of all sequences the tiles first that are the longest when causal, the last
+    // ones of the queries, the first ones of the keys
     const int n = keys ? a.nk : a.nq;
     const int per = static_cast<int>((static_cast<int64_t>(n) * mul + tile - 1) / tile);
-    s = static_cast<int>(slot % a.seqs);
-    r.tile = per - 1 - static_cast<int>(slot / a.seqs);
+    s = slot % a.seqs;
+    r.tile = keys ? slot / a.seqs : per - 1 - slot / a.seqs;
   } else {
     const int64_t total = keys ? a.total_k : a.total_q;
     const int lane = threadIdx.x & 63;
@@ -192,6 +209,14 @@ __device__ __forceinline__ Span find_span(const AttnArgs& a, int64_t slot, int m
   const int64_t rows = static_cast<int64_t>(keys ? r.lk : r.lq) * mul;
   if (r.tile < 0 || static_cast<int64_t>(r.tile) * tile >= rows) r.tile = -1;
   return r;
+}
+
+// The tiles [first, end) of number `split` of `nsplit` workgroups that share `tiles` tiles.
+__device__ __forceinline__ void split_range(int tiles, int nsplit, int split, int* first,
+                                            int* end) {
+  const int per = (tiles + nsplit - 1) / nsplit;
+  *first = split * per < tiles ? split * per : tiles;
+  *end = *first + per < tiles ? *first + per : tiles;
 }
 
 // ---------------------------------------------------------------------------
@@ -358,40 +383,27 @@ __device__ __forceinline__ void store_block(T* out, const f32x16& acc, int blk, 
   }
 }
 
-// Adds the infinities and NaN of an operand to a product whose weights are zero at masked
-// places, as the sum over the places that are not masked would have them: the product itself
-// was made with the operand's finite part, since 0 times infinity is NaN at masked places too.
-// w: weights (>= 0 or NaN), block of 32 summed rows x 32 lanes; seen(r): whether register row r
-// of the lane is not masked; frags(t): the operand's fragment of rows 16 t ...
-template <typename T, typename Seen, typename Frags>
-__device__ __forceinline__ void add_nonfinite(f32x16& acc, const f32x16& w, Seen seen,
-                                              Frags frags) {
-  typedef typename Elem<T>::frag F;
+// Adds the infinities and NaN of rows [r0, r1) (r0 <= r1; row_ptr(r): row r) to a result with
+// channels in its registers, for the rows that seen(r) of this lane: what was left out of a
+// product by Finite.  A weight at a place that is not masked is positive, or NaN and then the
+// result is NaN already, so a sum over the seen infinities and NaN is the product's.  Rare: plain
+// loads, one row at a time.
+template <typename T, int BLK, typename RowPtr, typename Seen>
+__device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[BLK], int r0, int r1, int hd,
+                                           RowPtr row_ptr, Seen seen) {
+  const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll 1
-  for (int kind = 0; kind < 4; ++kind) {
-    // 0: +inf under a weight, 1: -inf under a weight, 2: NaN, 3: an infinity under weight zero
-    f32x16 n = {};
+  for (int r = r0; r < r1; ++r) {
+    const T* p = row_ptr(r);
+    if (!seen(r)) continue;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const F f = frags(t);
-      F ind = zero_frag<F>(), has = zero_frag<F>();
+    for (int b = 0; b < BLK; ++b)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = static_cast<float>(f[j]), p = w[8 * t + j];
-        const bool i = kind == 0 ? x == INFINITY
-                       : kind == 1 ? x == -INFINITY
-                       : kind == 2 ? x != x
-                                   : fabsf(x) == INFINITY;
-        const bool h = seen(8 * t + j) && (kind == 2 || (kind == 3 ? p == 0.0f : p > 0.0f));
-        if (i) ind[j] = 1;
-        if (h) has[j] = 1;
+      for (int i = 0; i < 16; ++i) {
+        const int c = b * 32 + 8 * (i / 4) + 4 * g + i % 4;
+        const float x = c < hd ? to_f32(p[c]) : 0.0f;
+        if (!(fabsf(x) < INFINITY)) acc[b][i] += x;
       }
-      n = mma(ind, has, n);
-    }
-    const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __uint_as_float(0x7fc00000u);
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (n[r] > 0.0f) acc[r] += add;
   }
 }
 

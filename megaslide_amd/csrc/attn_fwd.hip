@@ -14,18 +14,10 @@ namespace {
 
 constexpr int kBN = 64;  // keys of a tile
 
-// Of `nsplit` workgroups along the keys, the tiles of number `split`.
-__device__ __forceinline__ void split_range(int tiles, int nsplit, int split, int* first,
-                                            int* end) {
-  const int per = (tiles + nsplit - 1) / nsplit;
-  *first = split * per < tiles ? split * per : tiles;
-  *end = *first + per < tiles ? *first + per : tiles;
-}
-
 template <typename T, int HD, int NW, bool VEC>
-__global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     const AttnArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
-    int nsplit, int64_t slots) {
+    int nsplit, int slots) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kBM = NW * 32, kNT = NW * 64, kKK = HD / 16, kBlk = HD / 32, kSB = kBN / 32;
   __shared__ __attribute__((aligned(16))) T s_k[2][kBN * HD];
@@ -33,11 +25,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
 
   // key head fastest: neighbours on the eight dies take different heads, and a head's tiles
   // keep to one die's L2 where the heads are a multiple of eight
-  int64_t id = blockIdx.x;
-  const int kvh = static_cast<int>(id % a.hk);
-  id /= a.hk;
-  const int split = static_cast<int>(id % nsplit);
-  const int64_t slot = a.cu_q == nullptr ? id / nsplit : slots - 1 - id / nsplit;
+  const unsigned id = blockIdx.x, hs = id / a.hk;
+  const int kvh = id - hs * a.hk;
+  const int sl = hs / nsplit, split = hs - sl * nsplit;
+  const int slot = a.cu_q == nullptr ? sl : slots - 1 - sl;
   const Span sp = find_span(a, slot, a.group, kBM, false);
   if (sp.tile < 0) return;
 
@@ -47,14 +38,14 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
   const int row0 = sp.tile * kBM + wave * 32;
   const int row = row0 + (lane & 31) < rows ? row0 + (lane & 31) : rows - 1;
   const int tok = row / a.group, head = kvh * a.group + row % a.group;
-  // keys before `limit` are seen by this lane's row, before `low` by every row of the wave,
-  // before `top` by some row of it, before `end` by some row of the workgroup
-  int limit = sp.lk, low = sp.lk, top = sp.lk, end = sp.lk;
+  // keys before `limit` are seen by this lane's row, before `top` by some row of the wave, before
+  // `all` by every row of the workgroup, before `end` by some row of it
+  int limit = sp.lk, all = sp.lk, top = sp.lk, end = sp.lk;
   if (a.causal) {
     const int last = (sp.tile + 1) * kBM < rows ? (sp.tile + 1) * kBM : rows;
     const int wlast = row0 + 32 < rows ? row0 + 32 : rows;
     limit = tok + 1 + shift;
-    low = (row0 < rows ? row0 : rows - 1) / a.group + 1 + shift;
+    all = sp.tile * kBM / a.group + 1 + shift;
     top = (wlast - 1) / a.group + 1 + shift;
     end = (last - 1) / a.group + 1 + shift;
     end = end > 0 ? end : 0;
@@ -90,11 +81,13 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
   }
   __syncthreads();
 
-  for (int t = first; t < stop; ++t) {
+  Finite<T> fin;
+  const auto step = [&](int t, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked_c)::value;
     const int buf = (t - first) & 1, k0 = t * kBN;
     const bool more = t + 1 < stop;
     if (more) load(t + 1);
-    if (row0 < rows && k0 < top) {
+    if (row0 < rows && (!kMasked || k0 < top)) {
       f32x16 s[kSB];
 #pragma unroll
       for (int b = 0; b < kSB; ++b) {
@@ -103,15 +96,14 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
         for (int i = 0; i < kKK; ++i)
           s[b] = mma(row_frag<T, HD>(s_k[buf], b * 32 + (lane & 31), i * 16 + g * 8), q[i], s[b]);
       }
-      const bool masked = k0 + kBN > low;
-      if (masked) {
+      if (kMasked) {
 #pragma unroll
         for (int b = 0; b < kSB; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (k0 + b * 32 + 8 * (r / 4) + 4 * g + r % 4 >= limit) s[b][r] = -INFINITY;
       }
-      float top_s = -INFINITY;
+      float top_s = s[0][0];
 #pragma unroll
       for (int b = 0; b < kSB; ++b)
 #pragma unroll
@@ -133,15 +125,6 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
           s[b][r] = __builtin_amdgcn_exp2f(s[b][r] * c - mc);
           l += s[b][r];
         }
-      // a value that is not finite must not reach rows that do not see its key
-      bool bad = false;
-      if (masked && a.causal) {
-#pragma unroll 1
-        for (int t2 = 0; t2 < kBN / 16; ++t2)
-#pragma unroll
-          for (int d = 0; d < kBlk; ++d) bad |= nonfinite(col_frag<T, HD>(s_v[buf], t2 * 16, d));
-        bad = __any(bad);
-      }
 #pragma unroll
       for (int b = 0; b < kSB; ++b)
 #pragma unroll
@@ -150,27 +133,26 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_fwd_kernel(
 #pragma unroll
           for (int d = 0; d < kBlk; ++d) {
             Frag v = col_frag<T, HD>(s_v[buf], b * 32 + t2 * 16, d);
-            if (bad) v = finite_part(v);
+            if (kMasked) v = fin(v);
             o[d] = mma(v, p, o[d]);
           }
         }
-      if (bad) {
-#pragma unroll
-        for (int b = 0; b < kSB; ++b)
-#pragma unroll
-          for (int d = 0; d < kBlk; ++d)
-            add_nonfinite<T>(
-                o[d], s[b],
-                [&](int r) { return k0 + b * 32 + 8 * (r / 4) + 4 * g + r % 4 < limit; },
-                [&](int t2) { return col_frag<T, HD>(s_v[buf], b * 32 + t2 * 16, d); });
-      }
     }
     if (more) {
       tk.store(s_k[buf ^ 1]);
       tv.store(s_v[buf ^ 1]);
     }
     __syncthreads();
-  }
+  };
+  int t = first, whole = all > 0 ? all / kBN : 0;  // tiles that every row sees whole
+  whole = whole < stop ? whole : stop;
+  for (; t < whole; ++t) step(t, std::false_type{});
+  const int cut = t;
+  for (; t < stop; ++t) step(t, std::true_type{});
+  if (__any(fin.bad()))
+    add_nonfinite<T>(
+        o, cut * kBN, stop * kBN < sp.lk ? stop * kBN : sp.lk, a.hd,
+        [=](int r) { return vp + r * a.vs; }, [=](int r) { return r < limit; });
 
   l = half_sum(l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -255,10 +237,10 @@ hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, float* l
   if (blocks == 0) return hipSuccess;
   if (vec)
     attn_fwd_kernel<T, HD, kNW, true>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, slots);
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, static_cast<int>(slots));
   else
     attn_fwd_kernel<T, HD, kNW, false>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, slots);
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, static_cast<int>(slots));
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || n == 1) return e;
   const int64_t rows = a.total_q * a.hq;
