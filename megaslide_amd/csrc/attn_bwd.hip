@@ -24,7 +24,7 @@ constexpr int kBQ = 64;          // rows of a passing tile (dK, dV)
 constexpr int kEnoughWgs = 1024;
 
 template <typename T, int HD, bool VEC>
-__global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_bwd_dq_kernel(
+__global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kernel(
     const AttnArgs a, const T* __restrict__ out, const T* __restrict__ dout,
     const float* __restrict__ lse, const float* __restrict__ dlse, T* __restrict__ dq,
     float2* __restrict__ stats, float* __restrict__ part, int nsplit, int slots) {
@@ -86,18 +86,35 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.ks + int64_t(kvh) * a.hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
   constexpr bool kTwo = sizeof(T) == 2;  // V double-buffered too (fp32: LDS holds three tiles)
-  Tile<T, HD, kBN, kNT, VEC> tk, tv;
-  const auto load = [&](int t) {
+  constexpr bool kDma = VEC && kTwo;
+  std::conditional_t<kDma, TileDma<HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
+  if constexpr (kDma) {
+    tk.init(a.hd, [&](int r) { return r * a.ks; });
+    tv.init(a.hd, [&](int r) { return r * a.vs; });
+  }
+  const auto load = [&](int t, int buf) __attribute__((always_inline)) {
     const int n = sp.lk - t * kBN;
     const T* kt = kp + static_cast<int64_t>(t) * kBN * a.ks;
     const T* vt = vp + static_cast<int64_t>(t) * kBN * a.vs;
-    tk.load([&](int r) { return kt + r * a.ks; }, n, a.hd);
-    tv.load([&](int r) { return vt + r * a.vs; }, n, a.hd);
+    if constexpr (kDma) {
+      tk.issue(kt, n * a.ks * 2, s_k[buf]);
+      tv.issue(vt, n * a.vs * 2, s_v[buf]);
+    } else {
+      tk.load([&](int r, int) { return kt + r * a.ks; }, n, a.hd);
+      tv.load([&](int r, int) { return vt + r * a.vs; }, n, a.hd);
+    }
+  };
+  const auto arrive = [&](int buf) __attribute__((always_inline)) {
+    if constexpr (kDma) {
+      dma_wait();
+    } else {
+      tk.store(s_k[buf]);
+      tv.store(s_v[kTwo ? buf : 0]);
+    }
   };
   if (first < stop) {
-    load(first);
-    tk.store(s_k[0]);
-    tv.store(s_v[0]);
+    load(first, 0);
+    arrive(0);
   }
   __syncthreads();
 
@@ -106,7 +123,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
     constexpr bool kMasked = decltype(masked_c)::value;
     const int buf = (t - first) & 1, vbuf = kTwo ? buf : 0, k0 = t * kBN;
     const bool more = t + 1 < stop;
-    if (more) load(t + 1);
+    if (more) load(t + 1, buf ^ 1);
     if (row0 < rows && (!kMasked || k0 < top)) {
 #pragma unroll
       for (int b = 0; b < kBN / 32; ++b) {
@@ -135,10 +152,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
       }
     }
     if (!kTwo) __syncthreads();
-    if (more) {
-      tk.store(s_k[buf ^ 1]);
-      tv.store(s_v[kTwo ? buf ^ 1 : 0]);
-    }
+    if (more) arrive(buf ^ 1);
     __syncthreads();
   };
   int t = first, whole = all > 0 ? all / kBN : 0;  // tiles that every row sees whole
@@ -208,40 +222,86 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
   for (int b = 0; b < kBlk; ++b) ak[b] = av[b] = f32x16{};
   const float c = a.scale * kLog2e;
 
-  Tile<T, HD, kBQ, kNT, VEC> tq, tg;
+  // A tile has as many whole tokens of the group's heads as 64 rows hold, so that every tile is
+  // laid out alike; groups of more than 64 heads (not VEC) divide for every row.
+  const int toks = VEC ? kBQ / a.group : 0, trows = VEC ? toks * a.group : kBQ;
+  constexpr bool kDma = VEC && sizeof(T) == 2;
+  std::conditional_t<kDma, TileDma<HD, kBQ, kNT>, Tile<T, HD, kBQ, kNT, VEC>> tq, tg;
+  const int64_t gs = static_cast<int64_t>(a.hq) * a.hd;
+  const T* qbase = static_cast<const T*>(a.q) + sp.q0 * a.qs + int64_t(kvh) * a.group * a.hd;
+  const T* gbase = dout + sp.q0 * gs + int64_t(kvh) * a.group * a.hd;
+  const float2* sbase = stats + sp.q0 * a.hq + kvh * a.group;
+  const auto row_off = [&](int r, int64_t stride) -> int64_t {
+    if (r >= trows) return -1;
+    const int tok = r / a.group;
+    return tok * stride + (r - tok * a.group) * a.hd;
+  };
+  const int64_t soff = tid < kBQ ? (tid < trows ? tid / a.group * static_cast<int64_t>(a.hq) +
+                                                      tid % a.group
+                                                : 0)
+                                 : 0;
+  int64_t qoff[kDma || !VEC ? 1 : decltype(tq)::kItems], goff[kDma || !VEC ? 1 : decltype(tq)::kItems];
+  if constexpr (kDma) {
+    tq.init(a.hd, [&](int r) { return row_off(r, a.qs); });
+    tg.init(a.hd, [&](int r) { return row_off(r, gs); });
+  } else if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < decltype(tq)::kItems; ++i) {
+      const int r = (tid + i * kNT) / decltype(tq)::kChunks;
+      qoff[i] = row_off(r, a.qs);
+      goff[i] = row_off(r, gs);
+    }
+  }
   float2 st;
-  const T* qbase = static_cast<const T*>(a.q) + sp.q0 * a.qs;
-  const auto load = [&](int t) {
-    const int r0 = t * kBQ, n = rows - r0;
-    tq.load([&](int r) {
-      const unsigned x = r0 + r, tok = x / static_cast<unsigned>(a.group);
-      return qbase + tok * a.qs + int64_t(kvh * a.group + (x - tok * a.group)) * a.hd;
-    }, n, a.hd);
-    tg.load([&](int r) {
-      const unsigned x = r0 + r, tok = x / static_cast<unsigned>(a.group);
-      return dout + ((sp.q0 + tok) * a.hq + kvh * a.group + (x - tok * a.group)) * a.hd;
-    }, n, a.hd);
+  const auto load = [&](int t, int buf) __attribute__((always_inline)) {
+    const int r0 = t * trows;
+    const int n = rows - r0 < trows ? rows - r0 : trows;
     st = make_float2(INFINITY, 0.0f);
-    if (tid < kBQ && tid < n) {
-      const unsigned x = r0 + tid, tok = x / static_cast<unsigned>(a.group);
-      st = stats[(sp.q0 + tok) * a.hq + kvh * a.group + (x - tok * a.group)];
+    if constexpr (VEC) {
+      const int64_t tok0 = static_cast<int64_t>(t) * toks;
+      const T* qt = qbase + tok0 * a.qs;
+      const T* gt = gbase + tok0 * gs;
+      if constexpr (kDma) {
+        const int64_t left = sp.lq - tok0;
+        tq.issue(qt, left * a.qs * 2, s_q[buf]);
+        tg.issue(gt, left * gs * 2, s_g[buf]);
+      } else {
+        tq.load([&](int, int i) { return qt + qoff[i]; }, n, a.hd);
+        tg.load([&](int, int i) { return gt + goff[i]; }, n, a.hd);
+      }
+      if (tid < n) st = sbase[tok0 * a.hq + soff];
+    } else {
+      const auto at = [&](int r, int64_t stride) {
+        const unsigned x = r0 + r, tok = x / static_cast<unsigned>(a.group);
+        return tok * stride + static_cast<int64_t>(x - tok * a.group) * a.hd;
+      };
+      tq.load([&](int r, int) { return qbase + at(r, a.qs); }, n, a.hd);
+      tg.load([&](int r, int) { return gbase + at(r, gs); }, n, a.hd);
+      if (tid < n) {
+        const unsigned x = r0 + tid, tok = x / static_cast<unsigned>(a.group);
+        st = sbase[static_cast<int64_t>(tok) * a.hq + (x - tok * a.group)];
+      }
     }
   };
-  const auto store = [&](int buf) {
-    tq.store(s_q[buf]);
-    tg.store(s_g[buf]);
+  const auto arrive = [&](int buf) __attribute__((always_inline)) {
     if (tid < kBQ) {
       s_lse[buf][tid] = st.x;
       s_delta[buf][tid] = st.y;
     }
+    if constexpr (kDma) {
+      dma_wait();
+    } else {
+      tq.store(s_q[buf]);
+      tg.store(s_g[buf]);
+    }
   };
   int t0, stop;
-  split_range((rows + kBQ - 1) / kBQ - begin / kBQ, nsplit, split, &t0, &stop);
-  t0 += begin / kBQ;
-  stop += begin / kBQ;
+  split_range((rows + trows - 1) / trows - begin / trows, nsplit, split, &t0, &stop);
+  t0 += begin / trows;
+  stop += begin / trows;
   if (t0 < stop) {
-    load(t0);
-    store(0);
+    load(t0, 0);
+    arrive(0);
   }
   __syncthreads();
 
@@ -250,11 +310,11 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
     constexpr bool kMasked = decltype(masked_c)::value;
     const int buf = kBufs == 2 ? (t - t0) & 1 : 0;
     const bool more = t + 1 < stop;
-    if (more) load(t + 1);
+    if (more) load(t + 1, kBufs == 2 ? buf ^ 1 : 0);
     if (key0 < sp.lk) {
 #pragma unroll
       for (int b = 0; b < kBQ / 32; ++b) {
-        const int r0 = t * kBQ + b * 32;
+        const int r0 = t * trows + b * 32;
         if (kMasked && r0 + 32 <= wfirst) continue;
         f32x16 s = {}, dp = {};
 #pragma unroll
@@ -293,19 +353,19 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
       }
     }
     if (kBufs == 1) __syncthreads();
-    if (more) store(kBufs == 2 ? buf ^ 1 : 0);
+    if (more) arrive(kBufs == 2 ? buf ^ 1 : 0);
     __syncthreads();
   };
-  int t = t0, cut = (all + kBQ - 1) / kBQ;  // tiles from `cut` on see every key
+  int t = t0, cut = (all + trows - 1) / trows;  // tiles from `cut` on see every key
   cut = cut < t0 ? t0 : cut < stop ? cut : stop;
   for (; t < cut; ++t) step(t, std::true_type{});
   for (; t < stop; ++t) step(t, std::false_type{});
   if (__any(fing.bad()))
     add_nonfinite<T>(
-        av, t0 * kBQ, cut * kBQ < rows ? cut * kBQ : rows, a.hd,
+        av, t0 * trows, cut * trows < rows ? cut * trows : rows, a.hd,
         [=](int r) {
           const int tok = r / a.group;
-          return dout + ((sp.q0 + tok) * a.hq + kvh * a.group + (r - tok * a.group)) * a.hd;
+          return gbase + tok * gs + static_cast<int64_t>(r - tok * a.group) * a.hd;
         },
         [=](int r) { return r >= first; });
   if (!mine) return;
@@ -447,7 +507,7 @@ size_t attn_bwd_ws_bytes(const msd_attn_desc& d) {
 
 hipError_t launch_attn_bwd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p,
                            void* ws, hipStream_t s) {
-  bool vec = attn_rows_aligned(a, d.dtype);
+  bool vec = attn_vec(d, a, true);
   for (const void* ptr : {p.out, p.dout, static_cast<const void*>(p.dq),
                           static_cast<const void*>(p.dk), static_cast<const void*>(p.dv)})
     vec = vec && reinterpret_cast<uintptr_t>(ptr) % 16 == 0;

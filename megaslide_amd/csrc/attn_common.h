@@ -84,23 +84,20 @@ __device__ __forceinline__ F zero_frag() {
 // enter those products by their finite part, and what was left out is noted in `seen_bad`
 // (nonzero) and added afterwards where it is seen.
 struct FiniteBf16 {
-  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-  u16x8 ok = {1, 1, 1, 1, 1, 1, 1, 1};
+  uint32_t found = 0;
 
   __device__ __forceinline__ bf16x8 operator()(const bf16x8& f) {
-    const u16x8 u = __builtin_bit_cast(u16x8, f);
-    // 1 where the exponent is not all ones
-    const u16x8 lim = 0x7f80, one = 1;
-    const u16x8 fin = __builtin_elementwise_min(
-        __builtin_elementwise_sub_sat(lim, static_cast<u16x8>(u & static_cast<uint16_t>(0x7fff))),
-        one);
-    ok &= fin;
-    return __builtin_bit_cast(bf16x8, static_cast<u16x8>(u * fin));
+    u32x4 u = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // a half's bit 15 where its exponent is all ones, then the half's mask
+      const uint32_t b = ((u[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      found |= b;
+      u[i] &= ~(b | (b - (b >> 15)));
+    }
+    return __builtin_bit_cast(bf16x8, u);
   }
-  __device__ __forceinline__ bool bad() const {
-    const u32x4 u = __builtin_bit_cast(u32x4, ok);
-    return (u[0] & u[1] & u[2] & u[3]) != 0x00010001u;
-  }
+  __device__ __forceinline__ bool bad() const { return found != 0; }
 };
 struct FiniteF32 {
   bool any = false;
@@ -259,7 +256,7 @@ struct Tile {
       const int row = item / kChunks, c = item % kChunks * E;
       u32x4 v = {0, 0, 0, 0};
       if (row < rows && row < ROWS && c < hd) {
-        const T* p = row_ptr(row) + c;
+        const T* p = row_ptr(row, i) + c;
         if (VEC) {
           v = *reinterpret_cast<const u32x4*>(p);
         } else if (sizeof(T) == 2) {
@@ -288,6 +285,55 @@ struct Tile {
     }
   }
 };
+
+// The same tile straight from memory to LDS, 16 bytes a lane, without registers on the way
+// (bf16).  A wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in
+// which chunk a lane reads.  A row at or past `rows` (of one stride each, or the last one of
+// row_off's) and channels at or past hd lie behind the buffer's end and arrive as zeros.
+template <int HD, int ROWS, int NT>
+struct TileDma {
+  static constexpr int kChunks = HD / 8;
+  static constexpr int kItems = ROWS * kChunks / NT;
+  static_assert(ROWS * kChunks % NT == 0, "whole loads");
+  uint32_t voff[kItems];
+
+  // row_off(r): element offset of row r from the tile's first, below 2^30; negative: no row
+  template <typename RowOff>
+  __device__ __forceinline__ void init(int hd, RowOff row_off) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int item = threadIdx.x + i * NT;
+      const int row = item / kChunks;
+      const int c = (item % kChunks ^ swz<bf16, HD>(row)) * 8;
+      const int64_t off = row_off(row);
+      voff[i] = off < 0 || c >= hd ? 0x80000000u : static_cast<uint32_t>(off + c) * 2;
+    }
+  }
+
+  // p: the tile's first row, the same in every lane; bytes: from p to the end of its last row
+  __device__ __forceinline__ void issue(const bf16* p, int64_t bytes, const bf16* lds) const {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint32_t n = bytes < 0 ? 0u : bytes > 0x7fffffff ? 0x7fffffffu : static_cast<uint32_t>(bytes);
+    u32x4 rsrc = {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu, n,
+                  0x00020000u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (const __attribute__((address_space(3))) bf16*)lds));
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      // writes LDS only: no register is an output (nothing else here uses m0); waited for by
+      // dma_wait
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :
+                   : "s"(base + wave + i * NT * 16), "v"(voff[i]), "s"(rsrc)
+                   : "memory");
+  }
+};
+
+// Waits for this wave's loads to LDS; a barrier afterwards makes them everyone's.
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // 8 channels c .. c + 7 (c a multiple of 8) of a tile's row.
 template <typename T, int HD>

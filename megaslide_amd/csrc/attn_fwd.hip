@@ -66,18 +66,37 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
   split_range((end + kBN - 1) / kBN, nsplit, split, &first, &stop);
   const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.ks + int64_t(kvh) * a.hd;
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
-  Tile<T, HD, kBN, kNT, VEC> tk, tv;
-  const auto load = [&](int t) {
+  // bf16 rows of 16-byte chunks go straight to LDS, others through registers
+  constexpr bool kDma = VEC && sizeof(T) == 2;
+  std::conditional_t<kDma, TileDma<HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
+  if constexpr (kDma) {
+    tk.init(a.hd, [&](int r) { return r * a.ks; });
+    tv.init(a.hd, [&](int r) { return r * a.vs; });
+  }
+  // starts tile t on its way to buffer `buf`, and ends it
+  const auto load = [&](int t, int buf) __attribute__((always_inline)) {
     const int n = sp.lk - t * kBN;
     const T* kt = kp + static_cast<int64_t>(t) * kBN * a.ks;
     const T* vt = vp + static_cast<int64_t>(t) * kBN * a.vs;
-    tk.load([&](int r) { return kt + r * a.ks; }, n, a.hd);
-    tv.load([&](int r) { return vt + r * a.vs; }, n, a.hd);
+    if constexpr (kDma) {
+      tk.issue(kt, n * a.ks * 2, s_k[buf]);
+      tv.issue(vt, n * a.vs * 2, s_v[buf]);
+    } else {
+      tk.load([&](int r, int) { return kt + r * a.ks; }, n, a.hd);
+      tv.load([&](int r, int) { return vt + r * a.vs; }, n, a.hd);
+    }
+  };
+  const auto arrive = [&](int buf) __attribute__((always_inline)) {
+    if constexpr (kDma) {
+      dma_wait();
+    } else {
+      tk.store(s_k[buf]);
+      tv.store(s_v[buf]);
+    }
   };
   if (first < stop) {
-    load(first);
-    tk.store(s_k[0]);
-    tv.store(s_v[0]);
+    load(first, 0);
+    arrive(0);
   }
   __syncthreads();
 
@@ -86,7 +105,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     constexpr bool kMasked = decltype(masked_c)::value;
     const int buf = (t - first) & 1, k0 = t * kBN;
     const bool more = t + 1 < stop;
-    if (more) load(t + 1);
+    if (more) load(t + 1, buf ^ 1);
     if (row0 < rows && (!kMasked || k0 < top)) {
       f32x16 s[kSB];
 #pragma unroll
@@ -138,10 +157,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
           }
         }
     }
-    if (more) {
-      tk.store(s_k[buf ^ 1]);
-      tv.store(s_v[buf ^ 1]);
-    }
+    if (more) arrive(buf ^ 1);
     __syncthreads();
   };
   int t = first, whole = all > 0 ? all / kBN : 0;  // tiles that every row sees whole
@@ -291,12 +307,14 @@ AttnArgs attn_args(const msd_attn_desc& d, const void* q, const void* k, const v
   return a;
 }
 
-bool attn_rows_aligned(const AttnArgs& a, int dtype) {
-  const int64_t e = dtype == MSD_BF16 ? 2 : 4;
+bool attn_vec(const msd_attn_desc& d, const AttnArgs& a, bool bwd) {
+  const int64_t e = d.dtype == MSD_BF16 ? 2 : 4;
   const auto ok = [&](const void* p, int64_t stride) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * e % 16 == 0;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * e % 16 == 0 &&
+           stride <= (int64_t(1) << 23);  // a tile's rows are 32-bit offsets
   };
-  return a.hd % 8 == 0 && ok(a.q, a.qs) && ok(a.k, a.ks) && ok(a.v, a.vs);
+  return a.hd % 8 == 0 && ok(a.q, a.qs) && ok(a.k, a.ks) && ok(a.v, a.vs) &&
+         (!bwd || (a.group <= 64 && int64_t(a.hq) * a.hd <= (int64_t(1) << 23)));
 }
 
 // Upper bound over both forms (packed or equal lengths): the descriptor does not say which.
@@ -310,7 +328,7 @@ size_t attn_fwd_ws_bytes(const msd_attn_desc& d) {
 
 hipError_t launch_attn_fwd(const msd_attn_desc& d, const AttnArgs& a, void* out, float* lse,
                            void* ws, hipStream_t s) {
-  const bool vec = attn_rows_aligned(a, d.dtype) && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool vec = attn_vec(d, a, false) && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   return d.dtype == MSD_BF16 ? launch_type<bf16>(d, a, out, lse, ws, vec, s)
                              : launch_type<float>(d, a, out, lse, ws, vec, s);
 }
