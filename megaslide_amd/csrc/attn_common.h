@@ -220,15 +220,15 @@ __device__ __forceinline__ void split_range(int tiles, int nsplit, int split, in
 // tiles
 // ---------------------------------------------------------------------------
 
-// XOR of a row's 16-byte chunks.  bf16: eight rows at one chunk (16-byte reads) and four rows
-// at one pair of chunks (transposing reads) lie in different banks; even, so that a pair stays
-// a pair.  fp32: eight rows at one chunk do.
+// XOR of a row's 16-byte chunks.  bf16: sixteen rows at one chunk (16-byte reads) and four rows
+// at four chunks (transposing reads) fill the 64 banks once.  fp32: eight rows at one chunk do.
 template <typename T, int HD>
 __device__ __forceinline__ int swz(int row) {
   if (sizeof(T) == 4) return row & 7;
-  if (HD == 128) return ((row & 3) << 2) | (((row >> 2) & 1) << 1);
-  if (HD == 64) return (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1);
-  return ((row >> 2) & 1) << 1;
+  const int k = (row >> 2) & 3;
+  if (HD == 128) return ((row & 3) << 2) | k;
+  if (HD == 64) return (((row >> 1) & 1) << 2) | k;
+  return k;
 }
 
 // Element offset of channel c (a multiple of a chunk's) of a tile's row.
@@ -357,9 +357,9 @@ __device__ __forceinline__ typename Elem<T>::frag col_frag(T* lds, int r0, int b
     const int row = r0 + 4 * g + ((l & 15) >> 2);
     const int c = blk * 32 + ((l >> 4) & 1) * 16 + (l & 3) * 4;
     const T* p = lds + at<T, HD>(row, c & ~7) + (c & 7);
-    // 8 rows further the XOR is the same
-    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p));
-    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + 8 * HD));
+    const T* q = lds + at<T, HD>(row + 8, c & ~7) + (c & 7);
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)p);
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)q);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   } else {
     const int c = blk * 32 + (l & 31);

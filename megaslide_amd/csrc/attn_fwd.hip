@@ -15,7 +15,7 @@ namespace {
 constexpr int kBN = 64;  // keys of a tile
 
 template <typename T, int HD, int NW, bool VEC>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) void attn_fwd_kernel(
     const AttnArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
     int nsplit, int slots) {
   typedef typename Elem<T>::frag Frag;
