@@ -29,7 +29,7 @@ struct AttnBwdPtrs {
 
 AttnArgs attn_args(const msd_attn_desc& d, const void* q, const void* k, const void* v,
                    const int32_t* cu_q, const int32_t* cu_k);
-// Whether rows of q, k, v are read in 16-byte chunks (the backward: and a tile of 64 rows holds
+// Whether rows of q, k, v are read in 16-byte chunks (the backward: and a tile of 32 rows holds
 // whole tokens of a group's heads); else element by element.
 bool attn_vec(const msd_attn_desc& d, const AttnArgs& a, bool bwd);
 int attn_max_head_dim();

@@ -20,14 +20,20 @@ constexpr int kNW = 4;
 constexpr int kNT = kNW * 64;
 constexpr int kTile = kNW * 32;  // stationary rows of a workgroup
 constexpr int kBN = 64;          // keys of a passing tile (dQ)
-constexpr int kBQ = 64;          // rows of a passing tile (dK, dV)
+// dK, dV of wide bf16 heads: two accumulators of 32 keys leave no registers for the keys' and the
+// values' fragments beside them at two waves a SIMD.  The values then stay in LDS, and the
+// passing tiles have 32 rows instead of 64, so that two workgroups still fit a compute unit.
+template <typename T, int HD>
+constexpr bool kWideOf = sizeof(T) == 2 && HD > 64;
+template <typename T, int HD>
+constexpr int kRowsOf = kWideOf<T, HD> ? 32 : 64;  // rows of a passing tile (dK, dV)
 constexpr int kEnoughWgs = 1024;
 
 template <typename T, int HD, bool VEC>
 __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kernel(
     const AttnArgs a, const T* __restrict__ out, const T* __restrict__ dout,
     const float* __restrict__ lse, const float* __restrict__ dlse, T* __restrict__ dq,
-    float2* __restrict__ stats, float* __restrict__ part, int nsplit, int slots) {
+    float2* __restrict__ stats, float* __restrict__ part, int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kKK = HD / 16, kBlk = HD / 32;
   __shared__ __attribute__((aligned(16))) T s_k[2][kBN * HD];
@@ -36,7 +42,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
   const int hs = blockIdx.x / static_cast<unsigned>(a.hk);
   const int kvh = blockIdx.x - hs * a.hk;
   const int id = hs / nsplit, split = hs - id * nsplit;
-  const Span sp = find_span(a, a.cu_q == nullptr ? id : slots - 1 - id, a.group, kTile, false);
+  const Span sp = find_span(a, id, a.group, kTile, false);
   if (sp.tile < 0) return;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5;
@@ -171,18 +177,27 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
 }
 
 template <typename T, int HD, bool VEC>
-__global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_bwd_dkv_kernel(
+__global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kernel(
     const AttnArgs a, const T* __restrict__ dout, const float2* __restrict__ stats,
     T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part, int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kKK = HD / 16, kBlk = HD / 32;
-  constexpr int kBufs = sizeof(T) == 2 ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) T s_q[kBufs][kBQ * HD];
-  __shared__ __attribute__((aligned(16))) T s_g[kBufs][kBQ * HD];
-  __shared__ __attribute__((aligned(16))) float s_lse[kBufs][kBQ];
-  __shared__ __attribute__((aligned(16))) float s_delta[kBufs][kBQ];
+  constexpr int kBufs = sizeof(T) == 2 ? 2 : 1, kBQ = kRowsOf<T, HD>;
+  constexpr bool kWide = kWideOf<T, HD>;
+  // the tiles that loads fill directly come first: such loads reach 64 KB of LDS
+  __shared__ struct {
+    alignas(16) T q[kBufs][kBQ * HD];
+    alignas(16) T g[kBufs][kBQ * HD];
+    alignas(16) T v[kWide ? kTile * HD : 8];
+    alignas(16) float lse[kBufs][kBQ];
+    alignas(16) float delta[kBufs][kBQ];
+  } sm;
+  auto& s_q = sm.q;
+  auto& s_g = sm.g;
+  auto& s_v = sm.v;
+  auto& s_lse = sm.lse;
+  auto& s_delta = sm.delta;
 
-  // first tiles first: causal ones have the most rows
   const int hs = blockIdx.x / static_cast<unsigned>(a.hk);
   const int kvh = blockIdx.x - hs * a.hk;
   const int id = hs / nsplit, split = hs - id * nsplit;
@@ -211,19 +226,23 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
 
   const T* kp = static_cast<const T*>(a.k) + (sp.k0 + key) * a.ks + int64_t(kvh) * a.hd;
   const T* vp = static_cast<const T*>(a.v) + (sp.k0 + key) * a.vs + int64_t(kvh) * a.hd;
-  Frag kf[kKK], vf[kKK];
+  Frag kf[kKK], vf[kWide ? 1 : kKK];
 #pragma unroll
   for (int i = 0; i < kKK; ++i) {
     kf[i] = mem_frag<T, VEC>(kp, i * 16 + g * 8, a.hd);
-    vf[i] = mem_frag<T, VEC>(vp, i * 16 + g * 8, a.hd);
+    const Frag v = mem_frag<T, VEC>(vp, i * 16 + g * 8, a.hd);
+    if constexpr (kWide)  // (read by this wave only)
+      *reinterpret_cast<Frag*>(s_v + at<T, HD>(wave * 32 + (lane & 31), i * 16 + g * 8)) = v;
+    else
+      vf[i] = v;
   }
   f32x16 ak[kBlk], av[kBlk];
 #pragma unroll
   for (int b = 0; b < kBlk; ++b) ak[b] = av[b] = f32x16{};
   const float c = a.scale * kLog2e;
 
-  // A tile has as many whole tokens of the group's heads as 64 rows hold, so that every tile is
-  // laid out alike; groups of more than 64 heads (not VEC) divide for every row.
+  // A tile has as many whole tokens of the group's heads as its rows hold, so that every tile is
+  // laid out alike; groups of more than 32 heads (not VEC) divide for every row.
   const int toks = VEC ? kBQ / a.group : 0, trows = VEC ? toks * a.group : kBQ;
   constexpr bool kDma = VEC && sizeof(T) == 2;
   std::conditional_t<kDma, TileDma<HD, kBQ, kNT>, Tile<T, HD, kBQ, kNT, VEC>> tq, tg;
@@ -320,7 +339,12 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 && HD <= 64 ? 2 : 1) void attn_
 #pragma unroll
         for (int i = 0; i < kKK; ++i) {
           s = mma(row_frag<T, HD>(s_q[buf], b * 32 + (lane & 31), i * 16 + g * 8), kf[i], s);
-          dp = mma(row_frag<T, HD>(s_g[buf], b * 32 + (lane & 31), i * 16 + g * 8), vf[i], dp);
+          Frag v;
+          if constexpr (kWide)
+            v = row_frag<T, HD>(s_v, wave * 32 + (lane & 31), i * 16 + g * 8);
+          else
+            v = vf[i];
+          dp = mma(row_frag<T, HD>(s_g[buf], b * 32 + (lane & 31), i * 16 + g * 8), v, dp);
         }
         f32x16 p;
 #pragma unroll
@@ -428,7 +452,7 @@ Plan plan(const msd_attn_desc& d, bool packed) {
   Plan p;
   p.q_slots = d.total_q > 0 ? slots_of(d.total_q, d.num_seqs, group, packed) : 0;
   p.k_slots = d.total_k > 0 ? slots_of(d.total_k, d.num_seqs, 1, packed) : 0;
-  const int64_t keys = d.total_k / d.num_seqs / kBN, rows = d.total_q / d.num_seqs * group / kBQ;
+  const int64_t keys = d.total_k / d.num_seqs / kBN, rows = d.total_q / d.num_seqs * group / 64;
   p.q_split = splits(p.q_slots * d.num_kv_heads, keys);
   p.k_split = splits(p.k_slots * d.num_kv_heads, rows);
   return p;
@@ -465,8 +489,7 @@ hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtr
   if (pl.q_slots > 0) {
     attn_bwd_dq_kernel<T, HD, VEC>
         <<<static_cast<unsigned>(pl.q_slots * pl.q_split * a.hk), kNT, 0, s>>>(
-            a, static_cast<const T*>(p.out), dout, p.lse, p.dlse, dq, stats, part, pl.q_split,
-            static_cast<int>(pl.q_slots));
+            a, static_cast<const T*>(p.out), dout, p.lse, p.dlse, dq, stats, part, pl.q_split);
     if (pl.q_split > 1) add(pl.q_split, a.total_q * a.hq, dq, nullptr);
   }
   hipError_t e = hipGetLastError();

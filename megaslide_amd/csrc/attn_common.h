@@ -145,27 +145,81 @@ __device__ __forceinline__ int64_t bound_of(const int32_t* cu, int s, int64_t to
   return c < 0 ? 0 : (c > total ? total : c);
 }
 
+// Sum (or maximum) of a wave's values, in every lane's reach: lane 63 has it after the DPP steps
+// within rows of 16 lanes and the two broadcasts across them.
+template <bool MAX>
+__device__ __forceinline__ int wave_reduce(int x) {
+  const auto step = [&](int y) { x = MAX ? (x > y ? x : y) : x + y; };
+  step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The sequence and tile of work item `slot`, where a sequence of n rows (times `mul`) takes
-// tiles of `tile` rows.  Sequence s owns the slots from floor(mul cu[s] / tile) + s on: at least
-// as many as it has tiles, and their number is known on the host from the totals alone, so
-// lengths stay on the device.  Rows behind the last sequence make one more sequence without a
-// counterpart.  Offsets that are not in order or out of range give wrong rows, never rows
-// outside the tensors.  `keys`: tiles of keys, else of queries.
+// tiles of `tile` rows.  There are floor(mul total / tile) + sequences + 1 slots: at least as
+// many as tiles, and a number that is known on the host from the totals alone, so lengths stay
+// on the device.  Rows behind the last sequence make one more sequence without a counterpart.
+// Offsets that are not in order or out of range give wrong rows, never rows outside the tensors.
+// `keys`: tiles of keys, else of queries.
+//
+// Workgroups start in the order of their slots, so the tiles with the most work come first and
+// the last ones to end are short: with up to 63 sequences (one a lane) by what a causal mask
+// leaves of them, or by their sequence's length, each wave finds its tile with a few reductions.
+// More sequences keep their own order, sequence s from slot floor(mul cu[s] / tile) + s on.
 __device__ __forceinline__ Span find_span(const AttnArgs& a, int slot, int mul, int tile,
                                           bool keys) {
   Span r;
   const int32_t* cu = keys ? a.cu_k : a.cu_q;
+  const int64_t total = keys ? a.total_k : a.total_q;
+  const int lane = threadIdx.x & 63;
   int s;
   if (cu == nullptr) {
-    // equal lengths: of all sequences the tiles first that are the longest when causal, the last
-    // ones of the queries, the first ones of the keys
     const int n = keys ? a.nk : a.nq;
     const int per = static_cast<int>((static_cast<int64_t>(n) * mul + tile - 1) / tile);
     s = slot % a.seqs;
     r.tile = keys ? slot / a.seqs : per - 1 - slot / a.seqs;
+  } else if (a.seqs < 64) {
+    const int64_t c0 = lane < a.seqs ? bound_of(cu, lane, total) : 0;
+    const int64_t c1 = lane < a.seqs ? bound_of(cu, lane + 1, total) : 0;
+    const int len = static_cast<int>(c1 > c0 ? c1 - c0 : 0);
+    const int nt = static_cast<int>((static_cast<int64_t>(len) * mul + tile - 1) / tile);
+    const int all = wave_reduce<false>(nt);
+    if (slot >= all) {
+      s = a.seqs;
+      r.tile = slot - all;
+    } else if (a.causal) {
+      // tiles by levels, from the highest: level v has tile v of the queries (the last - v of
+      // the keys) of every sequence that has so many
+      const int most = wave_reduce<true>(nt);
+      int lo = 0, hi = most - 1, above = 0;  // the lowest level with at most `slot` tiles above
+      while (lo < hi) {
+        const int v = (lo + hi) / 2;
+        if (wave_reduce<false>(nt > v + 1 ? nt - v - 1 : 0) <= slot)
+          hi = v;
+        else
+          lo = v + 1;
+      }
+      above = wave_reduce<false>(nt > lo + 1 ? nt - lo - 1 : 0);
+      uint64_t with = __ballot(nt > lo);
+      for (int k = slot - above; k > 0; --k) with &= with - 1;
+      s = __builtin_ctzll(with | (uint64_t(1) << 63));
+      r.tile = keys ? __builtin_amdgcn_readlane(nt, s) - 1 - lo : lo;
+    } else {
+      int before = 0;  // tiles of longer sequences, and of earlier ones of the same length
+      for (int i = 0; i < a.seqs; ++i) {
+        const int l = __builtin_amdgcn_readlane(len, i);
+        if (l > len || (l == len && i < lane)) before += __builtin_amdgcn_readlane(nt, i);
+      }
+      const uint64_t here = __ballot(lane < a.seqs && slot >= before && slot < before + nt);
+      s = __builtin_ctzll(here | (uint64_t(1) << 63));
+      r.tile = slot - __builtin_amdgcn_readlane(before, s);
+    }
+    s = s < a.seqs ? s : a.seqs;
   } else {
-    const int64_t total = keys ? a.total_k : a.total_q;
-    const int lane = threadIdx.x & 63;
     int lo = 0, n = a.seqs + 1;  // the answer is in [lo, lo + n)
     int64_t first = 0;           // its first slot
     while (n > 1) {
@@ -293,8 +347,8 @@ struct Tile {
 template <int HD, int ROWS, int NT>
 struct TileDma {
   static constexpr int kChunks = HD / 8;
-  static constexpr int kItems = ROWS * kChunks / NT;
-  static_assert(ROWS * kChunks % NT == 0, "whole loads");
+  static constexpr int kItems = (ROWS * kChunks + NT - 1) / NT;
+  static_assert(ROWS * kChunks % 64 == 0, "whole waves");
   uint32_t voff[kItems];
 
   // row_off(r): element offset of row r from the tile's first, below 2^30; negative: no row
@@ -322,13 +376,15 @@ struct TileDma {
         (const __attribute__((address_space(3))) bf16*)lds));
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
 #pragma unroll
-    for (int i = 0; i < kItems; ++i)
+    for (int i = 0; i < kItems; ++i) {
+      if (ROWS * kChunks % NT != 0 && wave + i * NT * 16 >= ROWS * HD * 2) break;
       // writes LDS only: no register is an output (nothing else here uses m0); waited for by
       // dma_wait
       asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :
                    : "s"(base + wave + i * NT * 16), "v"(voff[i]), "s"(rsrc)
                    : "memory");
+    }
   }
 };
 

@@ -17,7 +17,7 @@ constexpr int kBN = 64;  // keys of a tile
 template <typename T, int HD, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) void attn_fwd_kernel(
     const AttnArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
-    int nsplit, int slots) {
+    int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kBM = NW * 32, kNT = NW * 64, kKK = HD / 16, kBlk = HD / 32, kSB = kBN / 32;
   __shared__ __attribute__((aligned(16))) T s_k[2][kBN * HD];
@@ -27,8 +27,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) v
   // keep to one die's L2 where the heads are a multiple of eight
   const unsigned id = blockIdx.x, hs = id / a.hk;
   const int kvh = id - hs * a.hk;
-  const int sl = hs / nsplit, split = hs - sl * nsplit;
-  const int slot = a.cu_q == nullptr ? sl : slots - 1 - sl;
+  const int slot = hs / nsplit, split = hs - slot * nsplit;
   const Span sp = find_span(a, slot, a.group, kBM, false);
   if (sp.tile < 0) return;
 
@@ -253,10 +252,10 @@ hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, float* l
   if (blocks == 0) return hipSuccess;
   if (vec)
     attn_fwd_kernel<T, HD, kNW, true>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, static_cast<int>(slots));
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n);
   else
     attn_fwd_kernel<T, HD, kNW, false>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n, static_cast<int>(slots));
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || n == 1) return e;
   const int64_t rows = a.total_q * a.hq;
@@ -314,7 +313,7 @@ bool attn_vec(const msd_attn_desc& d, const AttnArgs& a, bool bwd) {
            stride <= (int64_t(1) << 23);  // a tile's rows are 32-bit offsets
   };
   return a.hd % 8 == 0 && ok(a.q, a.qs) && ok(a.k, a.ks) && ok(a.v, a.vs) &&
-         (!bwd || (a.group <= 64 && int64_t(a.hq) * a.hd <= (int64_t(1) << 23)));
+         (!bwd || (a.group <= 32 && int64_t(a.hq) * a.hd <= (int64_t(1) << 23)));
 }
 
 // Upper bound over both forms (packed or equal lengths): the descriptor does not say which.
