@@ -184,6 +184,19 @@ def dtype_code(dt: torch.dtype) -> int:
     raise TypeError(f"megaslide_amd: dtype {dt} not supported (float32 or bfloat16)")
 
 
+def launch(fn, what: str, index: int, *args) -> None:
+    """``fn(*args, stream)`` on device ``index`` and its current stream.  The device is switched
+    only where it is not the current one: small calls are bound by the host."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != 0:
+        check(rc, what)
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 

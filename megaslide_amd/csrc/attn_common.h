@@ -136,6 +136,7 @@ __device__ __forceinline__ float half_sum(float v) {
 struct Span {
   int64_t q0, k0;  // first row of the sequence's queries and keys
   int lq, lk;
+  int seq;         // the number of sequences: rows behind the last one
   int tile;        // tile of this workgroup within the sequence; < 0: no work
 };
 
@@ -237,6 +238,7 @@ __device__ __forceinline__ Span find_span(const AttnArgs& a, int slot, int mul, 
     r.tile = __builtin_amdgcn_readfirstlane(static_cast<int>(slot - first));
   }
   const bool tail = s >= a.seqs;
+  r.seq = s;
   if (a.cu_q != nullptr) {
     r.q0 = tail && keys ? 0 : bound_of(a.cu_q, s, a.total_q);
     int64_t e = tail ? (keys ? 0 : a.total_q) : bound_of(a.cu_q, s + 1, a.total_q);
@@ -344,6 +346,7 @@ struct Tile {
 // (bf16).  A wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in
 // which chunk a lane reads.  A row at or past `rows` (of one stride each, or the last one of
 // row_off's) and channels at or past hd lie behind the buffer's end and arrive as zeros.
+// NT: threads that share a tile, a workgroup's or (64) one wave's.
 template <int HD, int ROWS, int NT>
 struct TileDma {
   static constexpr int kChunks = HD / 8;
@@ -356,7 +359,7 @@ struct TileDma {
   __device__ __forceinline__ void init(int hd, RowOff row_off) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const int item = threadIdx.x + i * NT;
+      const int item = static_cast<int>(threadIdx.x) % NT + i * NT;
       const int row = item / kChunks;
       const int c = (item % kChunks ^ swz<bf16, HD>(row)) * 8;
       const int64_t off = row_off(row);
@@ -372,9 +375,10 @@ struct TileDma {
                   0x00020000u};
 #pragma unroll
     for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
-    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-        (const __attribute__((address_space(3))) bf16*)lds));
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) bf16*)lds)));
+    const uint32_t wave =
+        NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       if (ROWS * kChunks % NT != 0 && wave + i * NT * 16 >= ROWS * HD * 2) break;
@@ -388,8 +392,11 @@ struct TileDma {
   }
 };
 
-// Waits for this wave's loads to LDS; a barrier afterwards makes them everyone's.
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for this wave's loads to LDS but the N latest; a barrier afterwards makes them everyone's.
+template <int N = 0>
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 // 8 channels c .. c + 7 (c a multiple of 8) of a tile's row.
 template <typename T, int HD>

@@ -22,7 +22,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _require_device
 
 Tensor = torch.Tensor
 Positions = Union[Tensor, Sequence[int]]
@@ -41,13 +40,31 @@ def video_positions(video_shape: Sequence[int], device=None) -> Tensor:
     return torch.stack(torch.meshgrid(t, h, w, indexing="ij"), -1).reshape(-1, 3)
 
 
+def _device_index(*ts: Optional[Tensor]) -> int:
+    """The one device that all tensors are on."""
+    index = -1
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("megaslide_amd kernels run on ROCm devices only; got a tensor on "
+                               f"{t.device} (there is no CPU implementation)")
+        i = t.get_device()
+        if index < 0:
+            index = i
+        elif i != index:
+            raise RuntimeError(f"megaslide_amd: tensors on different devices ({index}, {i})")
+    return index
+
+
 def _rows(t: Tensor, name: str) -> Tuple[Tensor, int]:
     """``t`` ([N, D] or [B, N, D]) with unit channel stride and one stride between tokens, and
     that stride; a copy where its own layout is another."""
-    if t.dim() not in (2, 3):
-        raise ValueError(f"{name} must be [N, D] or [B, N, D], got {tuple(t.shape)}")
-    D = t.shape[-1]
-    if t.numel() == 0 or t.is_contiguous():
+    shape = t.shape
+    if len(shape) not in (2, 3):
+        raise ValueError(f"{name} must be [N, D] or [B, N, D], got {tuple(shape)}")
+    D = shape[-1]
+    if t.is_contiguous() or t.numel() == 0:
         return t, max(D, 1)
     if t.stride(-1) == 1 or D == 1:
         if t.dim() == 2 or t.shape[0] == 1:
@@ -73,92 +90,83 @@ def _split_heads(t: Tensor, heads: int, name: str) -> int:
 # rotation, norm
 # ---------------------------------------------------------------------------
 
-class _RopeCall:
-    """Validated arguments of one rotation and its C descriptor."""
+_Int4, _Int3 = ctypes.c_int32 * 4, ctypes.c_int32 * 3
+_NO_GRID = _Int3(0, 0, 0)
 
-    def __init__(self, what, q, k, weights, positions, num_heads, num_kv_heads, axes, theta, eps,
+
+class _RopeCall:
+    """Validated arguments of one rotation; ``args``: its C descriptor behind the strides."""
+
+    __slots__ = ("index", "weights", "pos", "head", "tail")
+
+    def __init__(self, what, q, k, wq, wk, positions, num_heads, num_kv_heads, axes, theta, eps,
                  interleaved, norm):
-        ts = [q, k, *weights]
-        if isinstance(positions, Tensor):
-            ts.append(positions)
-        self.dev = _require_device(*ts)
+        on_grid = not isinstance(positions, Tensor)
+        self.index = _device_index(q, k, wq, wk, None if on_grid else positions)
         hd = _split_heads(q, num_heads, what)
-        tokens = q.numel() // q.shape[-1]
-        self.shape = q.shape[:-1]
+        shape, dt = q.shape, q.dtype
+        n = shape[-2] if len(shape) > 1 else 0
         if k is not None:
-            if k.dtype != q.dtype:
-                raise TypeError(f"{what}: k is {k.dtype}, q is {q.dtype}")
-            if k.shape[:-1] != q.shape[:-1] or k.shape[-1] != num_kv_heads * hd:
-                raise ValueError(f"{what}: k must be {(*q.shape[:-1], num_kv_heads * hd)}, got "
+            if k.dtype != dt:
+                raise TypeError(f"{what}: k is {k.dtype}, q is {dt}")
+            if k.shape[:-1] != shape[:-1] or k.shape[-1] != num_kv_heads * hd:
+                raise ValueError(f"{what}: k must be {(*shape[:-1], num_kv_heads * hd)}, got "
                                  f"{tuple(k.shape)}")
-        self.weights, wdt = [], torch.float32
-        for name, w in zip(("q_weight", "k_weight"), weights):
+        wdt = None
+        for name, w in (("q_weight", wq), ("k_weight", wk)):
             if w is None:
-                self.weights.append(None)
                 continue
             if w.shape != (hd,):
                 raise ValueError(f"{what}: {name} must be {(hd,)}, got {tuple(w.shape)}")
-            if w.dtype not in (torch.float32, q.dtype):
-                raise TypeError(f"{what}: {name} is {w.dtype}, must be float32 or {q.dtype}")
-            self.weights.append(w.contiguous())
+            if w.dtype != torch.float32 and w.dtype != dt:
+                raise TypeError(f"{what}: {name} is {w.dtype}, must be float32 or {dt}")
+            if wdt is not None and w.dtype != wdt:
+                raise TypeError(f"{what}: q_weight and k_weight differ in dtype")
             wdt = w.dtype
-        if len({w.dtype for w in self.weights if w is not None}) > 1:
-            raise TypeError(f"{what}: q_weight and k_weight differ in dtype")
-        self.wdt = wdt
-        grid = (0, 0, 0)
-        n = q.shape[-2]
-        if isinstance(positions, Tensor):
-            if positions.dtype not in _lib.POS_DTYPES:
+        self.weights = (None if wq is None else wq.contiguous(),
+                        None if wk is None else wk.contiguous())
+        if on_grid:
+            grid = tuple(int(s) for s in positions)
+            if len(grid) != 3 or min(grid) < 0 or math.prod(grid) != n:
+                raise ValueError(f"{what}: a grid (T, H, W) of {n} tokens, got {grid}")
+            self.pos, n_axes, rows, pdt, grid = None, 3, n, _lib.POS_GRID, _Int3(*grid)
+        else:
+            pdt = _lib.POS_DTYPES.get(positions.dtype)
+            if pdt is None:
                 raise TypeError(f"{what}: positions are {positions.dtype}, must be one of "
                                 f"{[str(t) for t in _lib.POS_DTYPES]}")
             if positions.requires_grad:
                 raise ValueError(f"{what}: positions have no gradient")
-            if positions.dim() < 1 or positions.shape[:-1] not in ((n,), tuple(self.shape)):
+            ps = positions.shape
+            if len(ps) < 2 or (ps[:-1] != (n,) and ps[:-1] != shape[:-1]):
                 raise ValueError(f"{what}: positions must be [{n}, axes] or "
-                                 f"{(*self.shape, 'axes')}, got {tuple(positions.shape)}")
-            self.pos, n_axes = positions.contiguous(), positions.shape[-1]
-            rows, pdt = positions.numel() // max(n_axes, 1), _lib.POS_DTYPES[positions.dtype]
-        else:
-            grid = tuple(int(s) for s in positions)
-            if len(grid) != 3 or min(grid) < 0 or math.prod(grid) != n:
-                raise ValueError(f"{what}: a grid (T, H, W) of {n} tokens, got {grid}")
-            self.pos, n_axes, rows, pdt = None, 3, n, _lib.POS_GRID
+                                 f"{(*shape[:-1], 'axes')}, got {tuple(ps)}")
+            self.pos, n_axes, grid = positions.contiguous(), ps[-1], _NO_GRID
+            rows = n if len(ps) == 2 else n * ps[0]
         if axes is None:
-            axes = {1: (hd - hd % 2,), 3: video_axes(hd)}.get(n_axes)
-            if axes is None:
+            if n_axes != 1 and n_axes != 3:
                 raise ValueError(f"{what}: axes must be given for {n_axes} columns of positions")
+            axes = (hd - hd % 2,) if n_axes == 1 else video_axes(hd)
         axes = tuple(int(d) for d in axes)
         if len(axes) != n_axes or not 1 <= n_axes <= 4:
             raise ValueError(f"{what}: {len(axes)} axes, positions have {n_axes} columns (1 to 4)")
         if any(d < 0 or d % 2 for d in axes) or sum(axes) > hd:
             raise ValueError(f"{what}: axes {axes} must be even and at most {hd} channels together")
-        self.hd, self.tokens, self.heads = hd, tokens, (num_heads, 0 if k is None else num_kv_heads)
-        self.args = dict(theta=float(theta), dtype=_lib.dtype_code(q.dtype),
-                         weight_dtype=_lib.dtype_code(wdt), pos_dtype=pdt, n_axes=n_axes,
-                         axis_dims=(ctypes.c_int32 * 4)(*axes), interleaved=int(bool(interleaved)),
-                         norm=int(norm), eps=float(eps), grid=(ctypes.c_int32 * 3)(*grid),
-                         pos_rows=rows)
-
-    def desc(self, qs: int, ks: int) -> _lib.QkRopeDesc:
-        return _lib.QkRopeDesc(tokens=self.tokens, q_stride=qs, k_stride=ks,
-                               q_heads=self.heads[0], k_heads=self.heads[1], head_dim=self.hd,
-                               **self.args)
-
-    def empty(self, like: Tensor) -> Tensor:
-        return torch.empty(like.shape, dtype=like.dtype, device=self.dev)
+        self.head = (q.numel() // shape[-1], rows)
+        self.tail = (float(theta), num_heads, 0 if k is None else num_kv_heads, hd,
+                     _lib.dtype_code(dt), 0 if wdt is None else _lib.dtype_code(wdt), pdt, n_axes,
+                     _Int4(*axes), 1 if interleaved else 0, 1 if norm else 0, float(eps), grid)
 
     def forward(self, q, k):
         qr, qs = _rows(q, "q")
         kr, ks = (None, 0) if k is None else _rows(k, "k")
-        yq, yk = self.empty(q), None if k is None else self.empty(k)
+        yq, yk = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
         wq, wk = self.weights
-        desc = self.desc(qs, ks)
-        lib = _lib.load()
-        with torch.cuda.device(self.dev):
-            _lib.check(lib.msd_qk_rope_fwd(
-                ctypes.byref(desc), qr.data_ptr(), _lib.ptr(kr), _lib.ptr(wq), _lib.ptr(wk),
-                _lib.ptr(self.pos), yq.data_ptr(), _lib.ptr(yk), _lib.stream_handle(self.dev)),
-                "qk_rope_fwd")
+        desc = _lib.QkRopeDesc(*self.head, qs, ks, *self.tail)
+        ptr = _lib.ptr
+        _lib.launch(_lib.load().msd_qk_rope_fwd, "qk_rope_fwd", self.index, ctypes.byref(desc),
+                    qr.data_ptr(), ptr(kr), ptr(wq), ptr(wk), ptr(self.pos), yq.data_ptr(),
+                    ptr(yk))
         return yq, yk
 
     def backward(self, q, k, dyq, dyk, want_dw):
@@ -168,21 +176,18 @@ class _RopeCall:
         dyk = None if dyk is None else dyk.to(dt).contiguous()
         qr, qs = (None, dyq.shape[-1]) if q is None else _rows(q, "q")
         kr, ks = (None, 0 if dyk is None else dyk.shape[-1]) if k is None else _rows(k, "k")
-        dq, dk = self.empty(dyq), None if dyk is None else self.empty(dyk)
-        dw = [None if w is None or not want else torch.empty_like(w)
-              for w, want in zip(self.weights, want_dw)]
+        dq, dk = dyq.new_empty(dyq.shape), None if dyk is None else dyk.new_empty(dyk.shape)
         wq, wk = self.weights
-        desc = self.desc(qs, ks)
-        lib = _lib.load()
-        need = lib.msd_qk_rope_bwd_workspace_size(ctypes.byref(desc))
-        ws = torch.empty(need, dtype=torch.uint8, device=self.dev) if need else None
-        with torch.cuda.device(self.dev):
-            _lib.check(lib.msd_qk_rope_bwd(
-                ctypes.byref(desc), _lib.ptr(qr), _lib.ptr(kr), _lib.ptr(wq), _lib.ptr(wk),
-                _lib.ptr(self.pos), dyq.data_ptr(), _lib.ptr(dyk), dq.data_ptr(), _lib.ptr(dk),
-                _lib.ptr(dw[0]), _lib.ptr(dw[1]), _lib.ptr(ws), need,
-                _lib.stream_handle(self.dev)), "qk_rope_bwd")
-        return dq, dk, dw[0], dw[1]
+        dwq = torch.empty_like(wq) if wq is not None and want_dw[0] else None
+        dwk = torch.empty_like(wk) if wk is not None and want_dw[1] else None
+        desc = _lib.QkRopeDesc(*self.head, qs, ks, *self.tail)
+        lib, ptr, d = _lib.load(), _lib.ptr, ctypes.byref(desc)
+        need = lib.msd_qk_rope_bwd_workspace_size(d)
+        ws = dyq.new_empty(need, dtype=torch.uint8) if need else None
+        _lib.launch(lib.msd_qk_rope_bwd, "qk_rope_bwd", self.index, d, ptr(qr), ptr(kr), ptr(wq),
+                    ptr(wk), ptr(self.pos), dyq.data_ptr(), ptr(dyk), dq.data_ptr(), ptr(dk),
+                    ptr(dwq), ptr(dwk), ptr(ws), need)
+        return dq, dk, dwq, dwk
 
 
 class AxialRopeFunction(torch.autograd.Function):
@@ -225,7 +230,7 @@ def axial_rope(x: Tensor, positions: Positions, num_heads: int,
     None: all channels for one axis, ``video_axes(head_dim)`` for three.  Angles are held in 64
     bits.  Differentiable in x, once.
     """
-    call = _RopeCall("axial_rope", x, None, (None, None), positions, int(num_heads), 0, axes, theta,
+    call = _RopeCall("axial_rope", x, None, None, None, positions, int(num_heads), 0, axes, theta,
                      0.0, interleaved, False)
     if torch.is_grad_enabled() and x.requires_grad:
         return AxialRopeFunction.apply(x, call)
@@ -245,7 +250,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
     order.
     """
     num_kv_heads = int(num_heads if num_kv_heads is None else num_kv_heads)
-    call = _RopeCall("qk_norm_rope", q, k, (q_weight, k_weight), positions, int(num_heads),
+    call = _RopeCall("qk_norm_rope", q, k, q_weight, k_weight, positions, int(num_heads),
                      num_kv_heads, axes, theta, eps, interleaved, True)
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
@@ -260,21 +265,24 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
 class _AttnCall:
     """Validated arguments of one packed attention and its C descriptor."""
 
+    __slots__ = ("index", "q", "k", "v", "cu_q", "cu_k", "heads", "desc")
+
     def __init__(self, q, k, v, cu_q, cu_k, num_heads, num_kv_heads, causal, scale):
         what = "packed_attention"
-        self.dev = _require_device(q, k, v, cu_q, cu_k)
+        self.index = _device_index(q, k, v, cu_q, cu_k)
         hd = _split_heads(q, num_heads, what)
         if num_kv_heads < 1 or num_heads % num_kv_heads != 0:
             raise ValueError(f"{what}: num_heads={num_heads} must be a multiple of "
                              f"num_kv_heads={num_kv_heads}")
+        qsh, ksh, dt = q.shape, k.shape, q.dtype
         for name, t in (("k", k), ("v", v)):
-            if t.dtype != q.dtype:
-                raise TypeError(f"{what}: {name} is {t.dtype}, q is {q.dtype}")
-            if t.dim() != q.dim() or t.shape[-1] != num_kv_heads * hd:
+            if t.dtype != dt:
+                raise TypeError(f"{what}: {name} is {t.dtype}, q is {dt}")
+            if len(t.shape) != len(qsh) or t.shape[-1] != num_kv_heads * hd:
                 raise ValueError(f"{what}: {name} must have {num_kv_heads * hd} channels and as "
                                  f"many dimensions as q, got {tuple(t.shape)}")
-        if k.shape != v.shape:
-            raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        if ksh != v.shape:
+            raise ValueError(f"{what}: k {tuple(ksh)} and v {tuple(v.shape)} differ")
         self.q, qs = _rows(q, "q")
         self.k, ks = _rows(k, "k")
         self.v, vs = _rows(v, "v")
@@ -282,63 +290,55 @@ class _AttnCall:
         if cu_q is None:
             if cu_k is not None:
                 raise ValueError(f"{what}: cu_seqlens_k without cu_seqlens")
-            if q.dim() == 3:
-                if k.shape[0] != q.shape[0]:
-                    raise ValueError(f"{what}: batches {q.shape[0]} of q and {k.shape[0]} of k")
-                seqs = q.shape[0]
-            else:
-                seqs = 1
+            seqs = 1
+            if len(qsh) == 3:
+                seqs = qsh[0]
+                if ksh[0] != seqs:
+                    raise ValueError(f"{what}: batches {seqs} of q and {ksh[0]} of k")
         else:
-            if q.dim() != 2:
-                raise ValueError(f"{what}: packed sequences are [N, D], got {tuple(q.shape)}")
+            if len(qsh) != 2:
+                raise ValueError(f"{what}: packed sequences are [N, D], got {tuple(qsh)}")
             for name, c in (("cu_seqlens", cu_q), ("cu_seqlens_k", self.cu_k)):
                 if c.dtype != torch.int32 or c.dim() != 1 or c.numel() < 2 or not c.is_contiguous():
                     raise ValueError(f"{what}: {name} must be contiguous int32 of sequences + 1 "
                                      f"entries, got {c.dtype} {tuple(c.shape)}")
             seqs = cu_q.numel() - 1
-            if self.cu_k.numel() != seqs + 1:
-                raise ValueError(f"{what}: {seqs} sequences of q and {self.cu_k.numel() - 1} of k")
-            if cu_k is None and q.shape[0] != k.shape[0]:
-                raise ValueError(f"{what}: q has {q.shape[0]} rows and k {k.shape[0]}; give "
-                                 "cu_seqlens_k")
-        self.shape, self.hd, self.heads = q.shape, hd, num_heads
+            if cu_k is None:
+                if qsh[0] != ksh[0]:
+                    raise ValueError(f"{what}: q has {qsh[0]} rows and k {ksh[0]}; give "
+                                     "cu_seqlens_k")
+            elif cu_k.numel() != seqs + 1:
+                raise ValueError(f"{what}: {seqs} sequences of q and {cu_k.numel() - 1} of k")
+        self.heads = num_heads
         self.desc = _lib.AttnDesc(
-            q.numel() // q.shape[-1], k.numel() // k.shape[-1], qs, ks, vs, max(seqs, 1), num_heads,
-            num_kv_heads, hd, _lib.dtype_code(q.dtype), int(bool(causal)),
+            q.numel() // qsh[-1], k.numel() // ksh[-1], qs, ks, vs, max(seqs, 1), num_heads,
+            num_kv_heads, hd, _lib.dtype_code(dt), 1 if causal else 0,
             1.0 / math.sqrt(hd) if scale is None else float(scale))
 
     def forward(self, want_lse: bool):
-        q = self.q
-        out = torch.empty(self.shape, dtype=q.dtype, device=self.dev)
-        lse = (torch.empty((*self.shape[:-1], self.heads), dtype=torch.float32, device=self.dev)
-               if want_lse else None)
-        lib = _lib.load()
-        d = ctypes.byref(self.desc)
+        q, ptr = self.q, _lib.ptr
+        out = q.new_empty(q.shape)
+        lse = q.new_empty((*q.shape[:-1], self.heads), dtype=torch.float32) if want_lse else None
+        lib, d = _lib.load(), ctypes.byref(self.desc)
         need = lib.msd_attn_fwd_workspace_size(d)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.dev) if need else None
-        with torch.cuda.device(self.dev):
-            _lib.check(lib.msd_attn_fwd(
-                d, q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), _lib.ptr(self.cu_q),
-                _lib.ptr(self.cu_k), out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need,
-                _lib.stream_handle(self.dev)), "attn_fwd")
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        _lib.launch(lib.msd_attn_fwd, "attn_fwd", self.index, d, q.data_ptr(), self.k.data_ptr(),
+                    self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(), ptr(lse),
+                    ptr(ws), need)
         return out, lse
 
     def backward(self, out, lse, dout, dlse):
-        dt = self.q.dtype
-        out, lse, dout = out.contiguous(), lse.contiguous(), dout.to(dt).contiguous()
+        q, ptr = self.q, _lib.ptr
+        out, lse, dout = out.contiguous(), lse.contiguous(), dout.to(q.dtype).contiguous()
         dlse = None if dlse is None else dlse.to(torch.float32).contiguous()
-        dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=self.dev)
-                      for t in (self.q, self.k, self.v))
-        lib = _lib.load()
-        d = ctypes.byref(self.desc)
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, self.k, self.v))
+        lib, d = _lib.load(), ctypes.byref(self.desc)
         need = lib.msd_attn_bwd_workspace_size(d)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=self.dev)
-        with torch.cuda.device(self.dev):
-            _lib.check(lib.msd_attn_bwd(
-                d, self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), _lib.ptr(self.cu_q),
-                _lib.ptr(self.cu_k), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
-                _lib.ptr(dlse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need,
-                _lib.stream_handle(self.dev)), "attn_bwd")
+        ws = q.new_empty(max(need, 16), dtype=torch.uint8)
+        _lib.launch(lib.msd_attn_bwd, "attn_bwd", self.index, d, q.data_ptr(), self.k.data_ptr(),
+                    self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(),
+                    dout.data_ptr(), lse.data_ptr(), ptr(dlse), dq.data_ptr(), dk.data_ptr(),
+                    dv.data_ptr(), ws.data_ptr(), need)
         return dq, dk, dv
 
 

@@ -96,6 +96,47 @@ def test_long(dt, hd):
     check([300], [3001], 2, 1, hd, dt, False, scale=0.05)
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("lq,lk,heads,kv,hd", [
+    ([1] * 5, [1, 4000, 31, 33, 1025], 8, 2, 128),
+    ([1] * 3, [0, 2500, 257], 4, 4, 64),             # a sequence without keys
+    ([0, 2, 1], [700, 900, 1500], 6, 2, 96),         # as many tokens as sequences, not one each
+    ([3, 0, 0], [2, 900, 600], 4, 1, 80),            # two tokens that see no key when causal
+    ([1] * 70, [(i * 53) % 211 for i in range(70)], 32, 1, 32),  # more sequences than lanes
+    ([1] * 2, [700, 1300], 33, 1, 64),               # a group beyond one block's rows
+    ([1], [70001], 4, 1, 128),
+])
+def test_single_tokens(dt, lq, lk, heads, kv, hd):
+    """One new token each over caches (and calls that only look like it)."""
+    for causal in (True, False):
+        check(lq, lk, heads, kv, hd, dt, causal)
+
+
+def test_single_tokens_batched():
+    """[B, 1, D] over [B, M, D], views with a batch stride, NaN behind every cache's end."""
+    from megaslide_amd import packed_attention
+    g = gen(11)
+    B, M, heads, kv, hd = 6, 1003, 8, 2, 64
+    q, k, v = (randn(g, B, n, h * hd, dt=BF) for n, h in ((1, heads), (M, kv), (M, kv)))
+    want, err = attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), [1] * B, [M] * B,
+                          heads, kv, True)
+    out, lse = packed_attention(q, k, v, heads, kv, causal=True, return_lse=True)
+    assert_within(out.flatten(0, 1), want[0], err[0], "out")
+    assert_within(lse.flatten(0, 1), want[1], err[1], "lse")
+    # caches with room for more keys than they hold, packed by offsets of their own rows
+    room = 1500
+    big = [torch.full((B * room, kv * hd), math.nan, dtype=BF, device=DEV) for _ in range(2)]
+    for t, x in zip(big, (k, v)):
+        t.view(B, room, -1)[:, :M] = x
+    one = torch.ones(1, dtype=torch.int32, device=DEV)
+    for b in range(B):
+        cu_k = (torch.tensor([0, M], dtype=torch.int32, device=DEV))
+        rows = slice(b * room, (b + 1) * room)
+        got = packed_attention(q[b], big[0][rows], big[1][rows], heads, kv,
+                               torch.cat([one - 1, one]), cu_k, True)
+        assert_within(got, want[0][b:b + 1], err[0][b:b + 1], "with room")
+
+
 def test_seeded_shapes():
     """Random lengths, heads and sizes."""
     import random
