@@ -303,26 +303,28 @@ size_t msd_attn_fwd_workspace_size(const msd_attn_desc* desc);
  * total / num_seqs.  A row that sees no key has out = 0 and lse = -inf.
  * q [total_q, num_heads*head_dim], k, v [total_k, num_kv_heads*head_dim] with their
  * strides; out [total_q, num_heads*head_dim] contiguous; lse [total_q, num_heads]
- * fp32 or NULL.  What a row does not see (other sequences, later keys) does not
+ * fp32 or NULL.  out_rest (bf16 only, may be NULL) like out: what rounding took from
+ * out, rounded itself, for msd_attn_bwd.  What a row does not see (other sequences, later keys) does not
  * change it, infinities and NaN there included.
  */
 int msd_attn_fwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
-                 const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* workspace,
-                 size_t workspace_bytes, void* stream);
+                 const int32_t* cu_q, const int32_t* cu_k, void* out, void* out_rest, float* lse,
+                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of device workspace msd_attn_bwd needs for `desc`. */
 size_t msd_attn_bwd_workspace_size(const msd_attn_desc* desc);
 
 /*
  * Backward of msd_attn_fwd: out and lse are its results, dout (contiguous) the
- * gradient of out, dlse [total_q, num_heads] fp32 that of lse (NULL = 0).  dq, dk,
+ * gradient of out, out_rest msd_attn_fwd's or NULL (dq and dk of bf16 calls are then
+ * about a tenth further off), dlse [total_q, num_heads] fp32 that of lse (NULL = 0).  dq, dk,
  * dv are written, contiguous; rows in no sequence get zeros.  Sums are taken in a
  * fixed order: results repeat bit for bit.
  */
 int msd_attn_bwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
-                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* dout,
-                 const float* lse, const float* dlse, void* dq, void* dk, void* dv,
-                 void* workspace, size_t workspace_bytes, void* stream);
+                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* out_rest,
+                 const void* dout, const float* lse, const float* dlse, void* dq, void* dk,
+                 void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

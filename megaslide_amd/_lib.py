@@ -157,11 +157,11 @@ def load() -> ctypes.CDLL:
         lib.msd_attn_fwd_workspace_size.restype = ctypes.c_size_t
         lib.msd_attn_fwd_workspace_size.argtypes = [ctypes.POINTER(AttnDesc)]
         lib.msd_attn_fwd.restype = ctypes.c_int
-        lib.msd_attn_fwd.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 8 + [ctypes.c_size_t, _vp]
+        lib.msd_attn_fwd.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 9 + [ctypes.c_size_t, _vp]
         lib.msd_attn_bwd_workspace_size.restype = ctypes.c_size_t
         lib.msd_attn_bwd_workspace_size.argtypes = [ctypes.POINTER(AttnDesc)]
         lib.msd_attn_bwd.restype = ctypes.c_int
-        lib.msd_attn_bwd.argtypes = ([ctypes.POINTER(AttnDesc)] + [_vp] * 13 +
+        lib.msd_attn_bwd.argtypes = ([ctypes.POINTER(AttnDesc)] + [_vp] * 14 +
                                      [ctypes.c_size_t, _vp])
         v = lib.msd_abi_version()
         if v != ABI_VERSION:

@@ -458,8 +458,8 @@ size_t msd_attn_fwd_workspace_size(const msd_attn_desc* desc) {
 }
 
 int msd_attn_fwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
-                 const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* workspace,
-                 size_t workspace_bytes, void* stream) {
+                 const int32_t* cu_q, const int32_t* cu_k, void* out, void* out_rest, float* lse,
+                 void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_attn(desc);
   if (rc == MSD_OK) rc = check_lengths(desc, cu_q, cu_k);
   if (rc != MSD_OK) return rc;
@@ -469,12 +469,15 @@ int msd_attn_fwd(const msd_attn_desc* desc, const void* q, const void* k, const 
   if (rc == MSD_OK && desc->total_k > 0) rc = check_ptrs("attn_fwd(k, v)", a, {k, v});
   if (rc != MSD_OK) return rc;
   if (lse != nullptr && !aligned(lse, 4)) return fail(MSD_ERR_ALIGN, "attn_fwd: lse misaligned");
+  if (out_rest != nullptr && (!aligned(out_rest, a) || desc->dtype != MSD_BF16))
+    return fail(MSD_ERR_ARG, "attn_fwd: out_rest misaligned or not of bf16 results");
   const size_t need = msd::attn_fwd_ws_bytes(*desc);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(MSD_ERR_WORKSPACE, "attn_fwd: workspace of %zu bytes (16-aligned) needed, got %zu",
                 need, workspace == nullptr ? size_t(0) : workspace_bytes);
   return launch_status(msd::launch_attn_fwd(*desc, msd::attn_args(*desc, q, k, v, cu_q, cu_k), out,
-                                            lse, workspace, static_cast<hipStream_t>(stream)),
+                                            out_rest, lse, workspace,
+                                            static_cast<hipStream_t>(stream)),
                        "attn_fwd");
 }
 
@@ -484,9 +487,9 @@ size_t msd_attn_bwd_workspace_size(const msd_attn_desc* desc) {
 }
 
 int msd_attn_bwd(const msd_attn_desc* desc, const void* q, const void* k, const void* v,
-                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* dout,
-                 const float* lse, const float* dlse, void* dq, void* dk, void* dv,
-                 void* workspace, size_t workspace_bytes, void* stream) {
+                 const int32_t* cu_q, const int32_t* cu_k, const void* out, const void* out_rest,
+                 const void* dout, const float* lse, const float* dlse, void* dq, void* dk,
+                 void* dv, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_attn(desc);
   if (rc == MSD_OK) rc = check_lengths(desc, cu_q, cu_k);
   if (rc != MSD_OK) return rc;
@@ -498,11 +501,13 @@ int msd_attn_bwd(const msd_attn_desc* desc, const void* q, const void* k, const 
   if (rc == MSD_OK && desc->total_k > 0) rc = check_ptrs("attn_bwd(k, v)", a, {k, v, dk, dv});
   if (rc != MSD_OK) return rc;
   if (dlse != nullptr && !aligned(dlse, 4)) return fail(MSD_ERR_ALIGN, "attn_bwd: dlse misaligned");
+  if (out_rest != nullptr && (!aligned(out_rest, a) || desc->dtype != MSD_BF16))
+    return fail(MSD_ERR_ARG, "attn_bwd: out_rest misaligned or not of bf16 results");
   const size_t need = msd::attn_bwd_ws_bytes(*desc);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(MSD_ERR_WORKSPACE, "attn_bwd: workspace of %zu bytes (16-aligned) needed, got %zu",
                 need, workspace == nullptr ? size_t(0) : workspace_bytes);
-  const msd::AttnBwdPtrs p{out, dout, lse, dlse, dq, dk, dv};
+  const msd::AttnBwdPtrs p{out, out_rest, dout, lse, dlse, dq, dk, dv};
   return launch_status(msd::launch_attn_bwd(*desc, msd::attn_args(*desc, q, k, v, cu_q, cu_k), p,
                                             workspace, static_cast<hipStream_t>(stream)),
                        "attn_bwd");

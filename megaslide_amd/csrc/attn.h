@@ -19,6 +19,7 @@ struct AttnArgs {
 
 struct AttnBwdPtrs {
   const void* out;
+  const void* rest;  // what rounding took from out, or null
   const void* dout;
   const float* lse;
   const float* dlse;
@@ -35,8 +36,8 @@ bool attn_vec(const msd_attn_desc& d, const AttnArgs& a, bool bwd);
 int attn_max_head_dim();
 
 size_t attn_fwd_ws_bytes(const msd_attn_desc& d);
-hipError_t launch_attn_fwd(const msd_attn_desc& d, const AttnArgs& a, void* out, float* lse,
-                           void* ws, hipStream_t s);
+hipError_t launch_attn_fwd(const msd_attn_desc& d, const AttnArgs& a, void* out, void* rest,
+                           float* lse, void* ws, hipStream_t s);
 size_t attn_bwd_ws_bytes(const msd_attn_desc& d);
 hipError_t launch_attn_bwd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p,
                            void* ws, hipStream_t s);

@@ -31,8 +31,8 @@ constexpr int kEnoughWgs = 1024;
 
 template <typename T, int HD, bool VEC>
 __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kernel(
-    const AttnArgs a, const T* __restrict__ out, const T* __restrict__ dout,
-    const float* __restrict__ lse, const float* __restrict__ dlse, T* __restrict__ dq,
+    const AttnArgs a, const T* __restrict__ out, const T* __restrict__ rest,
+    const T* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ dlse, T* __restrict__ dq,
     float2* __restrict__ stats, float* __restrict__ part, int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kKK = HD / 16, kBlk = HD / 32;
@@ -75,6 +75,11 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
     const Frag o = mem_frag<T, VEC>(op, i * 16 + g * 8, a.hd);
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta += static_cast<float>(go[i][j]) * static_cast<float>(o[j]);
+    if (sizeof(T) == 2 && rest != nullptr) {
+      const Frag x = mem_frag<T, VEC>(rest + at_row * a.hd, i * 16 + g * 8, a.hd);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += static_cast<float>(go[i][j]) * static_cast<float>(x[j]);
+    }
   }
   delta = half_sum(delta);
   if (dlse != nullptr) delta -= dlse[at_row];
@@ -489,7 +494,7 @@ hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtr
   if (pl.q_slots > 0) {
     attn_bwd_dq_kernel<T, HD, VEC>
         <<<static_cast<unsigned>(pl.q_slots * pl.q_split * a.hk), kNT, 0, s>>>(
-            a, static_cast<const T*>(p.out), dout, p.lse, p.dlse, dq, stats, part, pl.q_split);
+            a, static_cast<const T*>(p.out), static_cast<const T*>(p.rest), dout, p.lse, p.dlse, dq, stats, part, pl.q_split);
     if (pl.q_split > 1) add(pl.q_split, a.total_q * a.hq, dq, nullptr);
   }
   hipError_t e = hipGetLastError();
@@ -531,7 +536,7 @@ size_t attn_bwd_ws_bytes(const msd_attn_desc& d) {
 hipError_t launch_attn_bwd(const msd_attn_desc& d, const AttnArgs& a, const AttnBwdPtrs& p,
                            void* ws, hipStream_t s) {
   bool vec = attn_vec(d, a, true);
-  for (const void* ptr : {p.out, p.dout, static_cast<const void*>(p.dq),
+  for (const void* ptr : {p.out, p.rest, p.dout, static_cast<const void*>(p.dq),
                           static_cast<const void*>(p.dk), static_cast<const void*>(p.dv)})
     vec = vec && reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
   return d.dtype == MSD_BF16 ? launch_type<bf16>(d, a, p, ws, vec, s)

@@ -492,6 +492,22 @@ __device__ __forceinline__ void store_block(T* out, const f32x16& acc, int blk, 
   }
 }
 
+// What rounding to bf16 took from a result, rounded itself: the backward's delta = sum(dO O)
+// multiplies every weight of its row, and from the rounded result alone it would be off by as
+// much as the weights' own rounding.
+template <typename T>
+__device__ __forceinline__ float rest_of(float v) {
+  return sizeof(T) == 2 ? v - static_cast<float>(static_cast<__bf16>(v)) : 0.0f;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_rest(T* out, const f32x16& acc, int blk, float f, int hd) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = rest_of<T>(acc[i] * f);
+  store_block<T, VEC>(out, r, blk, 1.0f, hd);
+}
+
 // Adds the infinities and NaN of rows [r0, r1) (r0 <= r1; row_ptr(r): row r) to a result with
 // channels in its registers, for the rows that seen(r) of this lane: what was left out of a
 // product by Finite.  A weight at a place that is not masked is positive, or NaN and then the

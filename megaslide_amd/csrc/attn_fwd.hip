@@ -16,8 +16,8 @@ constexpr int kBN = 64;  // keys of a tile
 
 template <typename T, int HD, int NW, bool VEC>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) void attn_fwd_kernel(
-    const AttnArgs a, T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
-    int nsplit) {
+    const AttnArgs a, T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse,
+    float* __restrict__ part, int nsplit) {
   typedef typename Elem<T>::frag Frag;
   constexpr int kBM = NW * 32, kNT = NW * 64, kKK = HD / 16, kBlk = HD / 32, kSB = kBN / 32;
   __shared__ __attribute__((aligned(16))) T s_k[2][kBN * HD];
@@ -184,6 +184,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) v
     T* op = out + at_row * a.hd;
 #pragma unroll
     for (int d = 0; d < kBlk; ++d) store_block<T, VEC>(op, o[d], d, inv, a.hd);
+    if (sizeof(T) == 2 && rest != nullptr) {
+#pragma unroll
+      for (int d = 0; d < kBlk; ++d)
+        store_rest<T, VEC>(rest + at_row * a.hd, o[d], d, inv, a.hd);
+    }
     if (lse != nullptr && g == 0) lse[at_row] = ls;
   }
 }
@@ -194,6 +199,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part,
                                                         int nsplit, int64_t rows, int hd,
                                                         int stride, T* __restrict__ out,
+                                                        T* __restrict__ rest,
                                                         float* __restrict__ lse) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
   const int lane = threadIdx.x & 63;
@@ -216,7 +222,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    if (lane + 64 * x < hd) out[row * hd + lane + 64 * x] = from_f32<T>(acc[x] * inv);
+    if (lane + 64 * x < hd) {
+      out[row * hd + lane + 64 * x] = from_f32<T>(acc[x] * inv);
+      if (rest != nullptr)
+        rest[row * hd + lane + 64 * x] = from_f32<T>(rest_of<T>(acc[x] * inv));
+    }
   if (lse != nullptr && lane == 0) lse[row] = sum == 0.0f ? -INFINITY : base + logf(sum);
 }
 
@@ -230,6 +240,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
 template <int HD>
 __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
                                                              bf16* __restrict__ out,
+                                                             bf16* __restrict__ rest,
                                                              float* __restrict__ lse,
                                                              float* __restrict__ part, int chunk,
                                                              int64_t units) {
@@ -389,6 +400,8 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
       } else {
         const int64_t r = (sp.q0 + tok) * a.hq + kvh * a.group + row;
         if (ch < a.hd) out[r * a.hd + ch] = from_f32<bf16>(acc);
+        if (ch < a.hd && rest != nullptr)
+          rest[r * a.hd + ch] = from_f32<bf16>(rest_of<bf16>(acc));
         if (ch == 0 && lse != nullptr) lse[r] = ls;
       }
     }
@@ -401,7 +414,7 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
 // without keys) become 0 and -inf.
 __global__ __launch_bounds__(256) void attn_join_tokens_kernel(
     const AttnArgs a, const float* __restrict__ part, int chunk, int64_t units, int hd_padded,
-    bf16* __restrict__ out, float* __restrict__ lse) {
+    bf16* __restrict__ out, bf16* __restrict__ rest, float* __restrict__ lse) {
   __shared__ float s_acc[4][128], s_sum[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.x / static_cast<unsigned>(a.hq);
@@ -448,8 +461,10 @@ __global__ __launch_bounds__(256) void attn_join_tokens_kernel(
   const int ch = threadIdx.x;
   const int64_t r = static_cast<int64_t>(row) * a.hq + head;
   if (ch < a.hd) {
-    const float v = s_acc[0][ch] + s_acc[1][ch] + s_acc[2][ch] + s_acc[3][ch];
-    out[r * a.hd + ch] = from_f32<bf16>(sum == 0.0f ? 0.0f : v / sum);
+    float v = s_acc[0][ch] + s_acc[1][ch] + s_acc[2][ch] + s_acc[3][ch];
+    v = sum == 0.0f ? 0.0f : v / sum;
+    out[r * a.hd + ch] = from_f32<bf16>(v);
+    if (rest != nullptr) rest[r * a.hd + ch] = from_f32<bf16>(rest_of<bf16>(v));
   }
   if (lse != nullptr && ch == 0) lse[r] = sum == 0.0f ? -INFINITY : base + logf(sum);
 }
@@ -493,26 +508,26 @@ int64_t token_units(const msd_attn_desc& d, int chunk) {
 }
 
 template <int HD>
-hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, bf16* out, float* lse,
-                         float* ws, int chunk, hipStream_t s) {
+hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, bf16* out, bf16* rest,
+                         float* lse, float* ws, int chunk, hipStream_t s) {
   const int64_t units = token_units(d, chunk);
   int64_t slots = units;
   if (a.cu_q == nullptr) slots = (d.total_k / d.num_seqs + chunk - 1) / chunk * d.num_seqs;
-  attn_tokens_kernel<HD><<<static_cast<unsigned>(slots * a.hk), 256, 0, s>>>(a, out, lse, ws,
-                                                                           chunk, units);
+  attn_tokens_kernel<HD><<<static_cast<unsigned>(slots * a.hk), 256, 0, s>>>(
+      a, out, rest, lse, ws, chunk, units);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   attn_join_tokens_kernel<<<static_cast<unsigned>(a.total_q * a.hq), 256, 0, s>>>(
-      a, ws, chunk, units, HD, out, lse);
+      a, ws, chunk, units, HD, out, rest, lse);
   return hipGetLastError();
 }
 
 template <typename T, int HD>
-hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, float* lse, float* ws,
-                     bool vec, hipStream_t s) {
+hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, T* rest, float* lse,
+                     float* ws, bool vec, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     const int chunk = vec ? token_chunk(d) : 0;
-    if (chunk > 0) return launch_tokens<HD>(d, a, out, lse, ws, chunk, s);
+    if (chunk > 0) return launch_tokens<HD>(d, a, out, rest, lse, ws, chunk, s);
   }
   const bool packed = a.cu_q != nullptr;
   const int n = splits(d, packed, kNW * 32);
@@ -521,28 +536,29 @@ hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, float* l
   if (blocks == 0) return hipSuccess;
   if (vec)
     attn_fwd_kernel<T, HD, kNW, true>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n);
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, rest, lse, ws, n);
   else
     attn_fwd_kernel<T, HD, kNW, false>
-        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, lse, ws, n);
+        <<<static_cast<unsigned>(blocks), kNW * 64, 0, s>>>(a, out, rest, lse, ws, n);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || n == 1) return e;
   const int64_t rows = a.total_q * a.hq;
   attn_join_kernel<T><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, s>>>(ws, n, rows, a.hd, HD,
-                                                                           out, lse);
+                                                                           out, rest, lse);
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch_type(const msd_attn_desc& d, const AttnArgs& a, void* out, float* lse, void* ws,
-                       bool vec, hipStream_t s) {
+hipError_t launch_type(const msd_attn_desc& d, const AttnArgs& a, void* out, void* rest,
+                       float* lse, void* ws, bool vec, hipStream_t s) {
   T* o = static_cast<T*>(out);
+  T* r = static_cast<T*>(rest);
   float* w = static_cast<float*>(ws);
   switch (padded_hd(a.hd)) {
-    case 32: return launch_hd<T, 32>(d, a, o, lse, w, vec, s);
-    case 64: return launch_hd<T, 64>(d, a, o, lse, w, vec, s);
-    case 96: return launch_hd<T, 96>(d, a, o, lse, w, vec, s);
-    default: return launch_hd<T, 128>(d, a, o, lse, w, vec, s);
+    case 32: return launch_hd<T, 32>(d, a, o, r, lse, w, vec, s);
+    case 64: return launch_hd<T, 64>(d, a, o, r, lse, w, vec, s);
+    case 96: return launch_hd<T, 96>(d, a, o, r, lse, w, vec, s);
+    default: return launch_hd<T, 128>(d, a, o, r, lse, w, vec, s);
   }
 }
 
@@ -597,11 +613,12 @@ size_t attn_fwd_ws_bytes(const msd_attn_desc& d) {
   return static_cast<size_t>(rows) * d.num_heads * (padded_hd(d.head_dim) + 1) * sizeof(float);
 }
 
-hipError_t launch_attn_fwd(const msd_attn_desc& d, const AttnArgs& a, void* out, float* lse,
-                           void* ws, hipStream_t s) {
-  const bool vec = attn_vec(d, a, false) && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  return d.dtype == MSD_BF16 ? launch_type<bf16>(d, a, out, lse, ws, vec, s)
-                             : launch_type<float>(d, a, out, lse, ws, vec, s);
+hipError_t launch_attn_fwd(const msd_attn_desc& d, const AttnArgs& a, void* out, void* rest,
+                           float* lse, void* ws, hipStream_t s) {
+  const bool vec = attn_vec(d, a, false) && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(rest) % 16 == 0;
+  return d.dtype == MSD_BF16 ? launch_type<bf16>(d, a, out, rest, lse, ws, vec, s)
+                             : launch_type<float>(d, a, out, nullptr, lse, ws, vec, s);
 }
 
 }  // namespace msd

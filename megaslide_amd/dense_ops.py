@@ -315,21 +315,24 @@ class _AttnCall:
             num_kv_heads, hd, _lib.dtype_code(dt), 1 if causal else 0,
             1.0 / math.sqrt(hd) if scale is None else float(scale))
 
-    def forward(self, want_lse: bool):
+    def forward(self, want_lse: bool, want_rest: bool = False):
+        """out, lse and what rounding took from out (bf16, for the backward), as wanted."""
         q, ptr = self.q, _lib.ptr
         out = q.new_empty(q.shape)
+        rest = q.new_empty(q.shape) if want_rest and q.dtype == torch.bfloat16 else None
         lse = q.new_empty((*q.shape[:-1], self.heads), dtype=torch.float32) if want_lse else None
         lib, d = _lib.load(), ctypes.byref(self.desc)
         need = lib.msd_attn_fwd_workspace_size(d)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         _lib.launch(lib.msd_attn_fwd, "attn_fwd", self.index, d, q.data_ptr(), self.k.data_ptr(),
-                    self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(), ptr(lse),
-                    ptr(ws), need)
-        return out, lse
+                    self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(), ptr(rest),
+                    ptr(lse), ptr(ws), need)
+        return out, lse, rest
 
-    def backward(self, out, lse, dout, dlse):
+    def backward(self, out, lse, rest, dout, dlse):
         q, ptr = self.q, _lib.ptr
         out, lse, dout = out.contiguous(), lse.contiguous(), dout.to(q.dtype).contiguous()
+        rest = None if rest is None or rest.numel() == 0 else rest.contiguous()
         dlse = None if dlse is None else dlse.to(torch.float32).contiguous()
         dq, dk, dv = (t.new_empty(t.shape) for t in (q, self.k, self.v))
         lib, d = _lib.load(), ctypes.byref(self.desc)
@@ -337,7 +340,7 @@ class _AttnCall:
         ws = q.new_empty(max(need, 16), dtype=torch.uint8)
         _lib.launch(lib.msd_attn_bwd, "attn_bwd", self.index, d, q.data_ptr(), self.k.data_ptr(),
                     self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(),
-                    dout.data_ptr(), lse.data_ptr(), ptr(dlse), dq.data_ptr(), dk.data_ptr(),
+                    ptr(rest), dout.data_ptr(), lse.data_ptr(), ptr(dlse), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), ws.data_ptr(), need)
         return dq, dk, dv
 
@@ -348,31 +351,34 @@ class _AttnCall:
 @torch.library.custom_op("megaslide::packed_attention", mutates_args=(), device_types="cuda")
 def _attn_fwd_op(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Optional[Tensor],
                  cu_seqlens_k: Optional[Tensor], num_heads: int, num_kv_heads: int, causal: bool,
-                 scale: Optional[float]) -> Tuple[Tensor, Tensor]:
-    """out like q and lse [..., num_heads] (fp32)."""
-    return _AttnCall(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal,
-                     scale).forward(want_lse=True)
+                 scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
+    """out like q, lse [..., num_heads] (fp32) and what rounding took from out (bf16, else
+    empty), which keeps the backward's sums of dout * out exact."""
+    out, lse, rest = _AttnCall(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal,
+                               scale).forward(want_lse=True, want_rest=True)
+    return out, lse, q.new_empty((0,)) if rest is None else rest
 
 
 @_attn_fwd_op.register_fake
 def _(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal, scale):
     return (q.new_empty(q.shape),
-            q.new_empty((*q.shape[:-1], num_heads), dtype=torch.float32))
+            q.new_empty((*q.shape[:-1], num_heads), dtype=torch.float32),
+            q.new_empty(q.shape if q.dtype == torch.bfloat16 else (0,)))
 
 
 @torch.library.custom_op("megaslide::packed_attention_bwd", mutates_args=(), device_types="cuda")
 def _attn_bwd_op(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Optional[Tensor],
-                 cu_seqlens_k: Optional[Tensor], out: Tensor, lse: Tensor, dout: Tensor,
-                 dlse: Optional[Tensor], num_heads: int, num_kv_heads: int, causal: bool,
-                 scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
+                 cu_seqlens_k: Optional[Tensor], out: Tensor, lse: Tensor, rest: Tensor,
+                 dout: Tensor, dlse: Optional[Tensor], num_heads: int, num_kv_heads: int,
+                 causal: bool, scale: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
     """dq, dk, dv."""
     return _AttnCall(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal,
-                     scale).backward(out, lse, dout, dlse)
+                     scale).backward(out, lse, rest, dout, dlse)
 
 
 @_attn_bwd_op.register_fake
-def _(q, k, v, cu_seqlens, cu_seqlens_k, out, lse, dout, dlse, num_heads, num_kv_heads, causal,
-      scale):
+def _(q, k, v, cu_seqlens, cu_seqlens_k, out, lse, rest, dout, dlse, num_heads, num_kv_heads,
+      causal, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
@@ -382,11 +388,12 @@ def _attn_setup(ctx, inputs, output):
     ctx.save_for_backward(*inputs[:5], *output)
 
 
-def _attn_backward(ctx, dout, dlse):
-    q, k, v, cu, cu_k, out, lse = ctx.saved_tensors
+def _attn_backward(ctx, dout, dlse, drest):
+    q, k, v, cu, cu_k, out, lse, rest = ctx.saved_tensors
     if dout is None:
         dout = torch.zeros_like(out)
-    return (*_attn_bwd_op(q, k, v, cu, cu_k, out, lse, dout, dlse, *ctx.args),) + (None,) * 6
+    return (*_attn_bwd_op(q, k, v, cu, cu_k, out, lse, rest, dout, dlse,
+                          *ctx.args),) + (None,) * 6
 
 
 _attn_fwd_op.register_autograd(_attn_backward, setup_context=_attn_setup)
@@ -417,10 +424,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, num_heads: int,
     num_heads = int(num_heads)
     num_kv_heads = int(num_heads if num_kv_heads is None else num_kv_heads)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        out, lse = torch.ops.megaslide.packed_attention(
+        out, lse, _ = torch.ops.megaslide.packed_attention(
             q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, bool(causal),
             None if scale is None else float(scale))
     else:
-        out, lse = _AttnCall(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal,
-                             scale).forward(want_lse=return_lse)
+        out, lse, _ = _AttnCall(q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal,
+                                scale).forward(want_lse=return_lse)
     return (out, lse) if return_lse else out

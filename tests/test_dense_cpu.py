@@ -86,9 +86,10 @@ def attn_desc(**kw):
     return _lib.AttnDesc(**d)
 
 
-def attn_fwd(desc, q=16, k=16, v=16, cu=16, cu_k=16, out=16, lse=16, ws=16, n=1 << 40):
+def attn_fwd(desc, q=16, k=16, v=16, cu=16, cu_k=16, out=16, rest=None, lse=16, ws=16,
+             n=1 << 40):
     return _lib.load().msd_attn_fwd(None if desc is None else ctypes.byref(desc), q, k, v, cu, cu_k,
-                                    out, lse, ws, n, None)
+                                    out, rest, lse, ws, n, None)
 
 
 @pytest.mark.parametrize("kw,code,needle", [
@@ -116,7 +117,7 @@ def test_attention_descriptors(kw, code, needle):
     d = attn_desc(**kw)
     assert attn_fwd(d) == code
     assert needle in lib.msd_last_error()
-    assert lib.msd_attn_bwd(ctypes.byref(d), *([16] * 13), 1 << 40, None) == code
+    assert lib.msd_attn_bwd(ctypes.byref(d), *([16] * 14), 1 << 40, None) == code
     assert lib.msd_attn_fwd_workspace_size(ctypes.byref(d)) == 0
     assert lib.msd_attn_bwd_workspace_size(ctypes.byref(d)) == 0
 
@@ -127,6 +128,8 @@ def test_attention_pointers_and_workspace():
     assert attn_fwd(attn_desc(), q=None) == -1 and b"NULL" in lib.msd_last_error()
     assert attn_fwd(attn_desc(), k=17) == -3
     assert attn_fwd(attn_desc(), lse=18) == -3
+    assert attn_fwd(attn_desc(), rest=17) == -1
+    assert attn_fwd(attn_desc(dtype=0), rest=16) == -1 and b"bf16" in lib.msd_last_error()
     assert attn_fwd(attn_desc(), cu=None) == -1 and b"together" in lib.msd_last_error()
     assert attn_fwd(attn_desc(), cu_k=18) == -3
     assert attn_fwd(attn_desc(total_q=25), cu=None, cu_k=None) == -1
@@ -142,7 +145,7 @@ def test_attention_pointers_and_workspace():
     d = attn_desc()
     need = lib.msd_attn_bwd_workspace_size(ctypes.byref(d))
     assert need >= 24 * 4 * 8
-    assert lib.msd_attn_bwd(ctypes.byref(d), *([16] * 13), need - 1, None) == -4
+    assert lib.msd_attn_bwd(ctypes.byref(d), *([16] * 14), need - 1, None) == -4
 
 
 def test_video_axes_and_positions():
