@@ -2,7 +2,8 @@
 
 Public surface:
   DeformableSlideAttention3D   drop-in for infinity/video/attention.py:19-273
-  DiTBlock, MLP                drop-ins for infinity/video/model.py:21-117 around it
+  DenseAttention3D             dense attention with rotary (time, height, width) positions
+  DiTBlock, MLP                drop-ins for infinity/video/model.py:21-117 around them
   dsa3d_core                   fused attention core (autograd; the custom
                                operator torch.ops.megaslide.dsa3d_core)
   axial_rope                   rotary positions with several axes (autograd)
@@ -17,14 +18,15 @@ Public surface:
                                ... and every GEMM's outputs
 """
 
-from .attention import DeformableSlideAttention3D
+from .attention import DeformableSlideAttention3D, DenseAttention3D
 from .block import MLP, DiTBlock, checkpoint_keep_core, checkpoint_keep_gemms
 from .dense_ops import (axial_rope, packed_attention, qk_norm_rope, video_axes,
                         video_positions)
 from .ops import (DwConv3dFunction, dsa3d_core, dwconv3d, keep_core_context, keep_core_policy,
                   keep_gemms_context, keep_gemms_policy)
 
-__all__ = ["DeformableSlideAttention3D", "DiTBlock", "MLP", "DwConv3dFunction", "axial_rope",
-           "dsa3d_core", "dwconv3d", "packed_attention", "qk_norm_rope", "video_axes",
-           "video_positions", "keep_core_policy", "keep_core_context", "checkpoint_keep_core",
-           "keep_gemms_policy", "keep_gemms_context", "checkpoint_keep_gemms"]
+__all__ = ["DeformableSlideAttention3D", "DenseAttention3D", "DiTBlock", "MLP",
+           "DwConv3dFunction", "axial_rope", "dsa3d_core", "dwconv3d", "packed_attention",
+           "qk_norm_rope", "video_axes", "video_positions", "keep_core_policy",
+           "keep_core_context", "checkpoint_keep_core", "keep_gemms_policy",
+           "keep_gemms_context", "checkpoint_keep_gemms"]

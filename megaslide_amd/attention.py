@@ -1,4 +1,5 @@
-"""Drop-in ``DeformableSlideAttention3D`` running on the gfx950 HIP kernels.
+"""Drop-in ``DeformableSlideAttention3D`` running on the gfx950 HIP kernels, and
+``DenseAttention3D``, dense attention of the same shape of module.
 
 Same constructor arguments, submodule names, parameter names/shapes/order,
 default initialisation and ``forward(x, video_shape, extra_kv=None)`` signature
@@ -21,6 +22,11 @@ What runs where:
     PyTorch GEMMs; the G extra keys and values join every query's taps in the
     HIP core's softmax (forward and backward, their gradients included).
 
+``DenseAttention3D`` attends to every token instead of a window around each (the
+reference's dense baseline, infinity/video/baselines.py): projections in PyTorch,
+the norm of queries and keys with their rotation by (time, height, width), and
+attention over packed sequences in HIP kernels.
+
 There is no CPU path: on CPU tensors ``forward`` raises.
 """
 
@@ -33,6 +39,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from .dense_ops import Positions, axial_rope, packed_attention, qk_norm_rope
 from .ops import dsa3d_core, dwconv3d
 
 
@@ -123,3 +130,66 @@ class DeformableSlideAttention3D(nn.Module):
                           extra_v=ev, dkv_accum=self.dkv_accum)
         return torch.addmm(dw.reshape(B * N, D), attn.reshape(B * N, D),
                            self.out_proj.weight.t()).view(B, N, D)
+
+
+class DenseAttention3D(nn.Module):
+    """Attention of every video token to every other, with rotary (time, height, width)
+    positions; ``forward(x, video_shape)`` as the deformable module's, so that a block can hold
+    either.
+
+    Args:
+        hidden_size: Hidden dimension D.
+        num_heads: Number of query heads.
+        num_kv_heads: Number of key and value heads (default: num_heads).
+        qk_norm: RMS norm of each head of queries and keys, with one weight per channel.
+        causal: Tokens see themselves and earlier ones only.
+        axes: Channels of a head turned by each axis of the positions (default: video_axes).
+        theta: Base of the rotation's frequencies.
+    """
+
+    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: Optional[int] = None,
+                 qk_norm: bool = True, causal: bool = False,
+                 axes: Optional[Tuple[int, ...]] = None, theta: float = 10000.0):
+        super().__init__()
+        num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        assert hidden_size % num_heads == 0, "hidden_size must be divisible by num_heads"
+        assert num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads"
+        self.hidden_size = hidden_size
+        self.num_heads = num_heads
+        self.num_kv_heads = num_kv_heads
+        self.head_dim = hidden_size // num_heads
+        self.causal = causal
+        self.axes = axes
+        self.theta = theta
+        kv = num_kv_heads * self.head_dim
+        self.q_proj = nn.Linear(hidden_size, hidden_size, bias=True)
+        self.k_proj = nn.Linear(hidden_size, kv, bias=True)
+        self.v_proj = nn.Linear(hidden_size, kv, bias=True)
+        self.out_proj = nn.Linear(hidden_size, hidden_size, bias=True)
+        self.q_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+
+    def forward(self, x: Tensor, video_shape: Optional[Tuple[int, int, int]] = None,
+                positions: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None) -> Tensor:
+        """x [B, N, D] with its video_shape (T, H, W); or x [N, D] of clips packed one after the
+        other, with the positions [N, axes] of its tokens and the clips' offsets cu_seqlens
+        (int32, clips + 1; default: one clip)."""
+        if x.device.type != "cuda":
+            raise RuntimeError("megaslide_amd.DenseAttention3D runs on ROCm devices only (HIP "
+                               "kernels; no CPU implementation)")
+        if (video_shape is None) == (positions is None):
+            raise ValueError("give video_shape or positions")
+        pos: Positions = video_shape if positions is None else positions
+        q, k, v = self.q_proj(x), self.k_proj(x), self.v_proj(x)
+        if self.q_norm is not None:
+            wq, wk = self.q_norm, self.k_norm
+            if wq.dtype not in (torch.float32, q.dtype):
+                wq, wk = wq.to(q.dtype), wk.to(q.dtype)
+            q, k = qk_norm_rope(q, k, wq, wk, pos, self.num_heads, self.num_kv_heads, self.axes,
+                                self.theta)
+        else:
+            q = axial_rope(q, pos, self.num_heads, self.axes, self.theta)
+            k = axial_rope(k, pos, self.num_kv_heads, self.axes, self.theta)
+        out = packed_attention(q, k, v, self.num_heads, self.num_kv_heads, cu_seqlens,
+                               causal=self.causal)
+        return self.out_proj(out)

@@ -48,13 +48,17 @@ class MLP(nn.Module):
 
 
 class DiTBlock(nn.Module):
-    """Pre-LayerNorm 3D-DSA and MLP with residuals (model.py:40-117)."""
+    """Pre-LayerNorm 3D-DSA and MLP with residuals (model.py:40-117).
 
-    def __init__(self, config):
+    ``attn``: another attention module in the place of 3D-DSA, called as
+    ``attn(x, video_shape)``; ``DenseAttention3D`` for a block that attends densely (the
+    reference's dense baseline, infinity/video/baselines.py)."""
+
+    def __init__(self, config, attn: Optional[nn.Module] = None):
         super().__init__()
         self.config = config
         self.norm1 = nn.LayerNorm(config.hidden_size, eps=1e-6)
-        self.attn = DeformableSlideAttention3D(
+        self.attn = attn if attn is not None else DeformableSlideAttention3D(
             hidden_size=config.hidden_size,
             num_heads=config.num_heads,
             kernel_size=tuple(config.dsa_kernel_size),
