@@ -477,13 +477,16 @@ int64_t q_slots(const msd_attn_desc& d, bool packed, int tile) {
   return d.total_q * group / tile + d.num_seqs + 1;
 }
 
-// Workgroups along the keys: enough that the launch fills the 256 compute units several times,
-// each with 256 keys at least of a sequence of mean length.
+// Workgroups along the keys: enough that the launch fills the 256 compute units, several times in
+// bf16, where two to four workgroups share one and sequences differ, each with 256 keys at least
+// of a sequence of mean length.  (Two fp32 clips of 2,048 tokens, 4 heads x 64: 164 us whole, 106
+// in two parts, 114 in four, 128 in eight.)
 int splits(const msd_attn_desc& d, bool packed, int tile) {
   const int64_t wgs = q_slots(d, packed, tile) * d.num_kv_heads;
-  if (wgs == 0 || wgs >= 512) return 1;
+  const int64_t enough = d.dtype == MSD_BF16 ? 1024 : 256;
+  if (wgs == 0 || wgs >= (d.dtype == MSD_BF16 ? 512 : 256)) return 1;
   const int64_t mean = d.total_k / d.num_seqs;
-  int64_t n = (1024 + wgs - 1) / wgs;
+  int64_t n = (enough + wgs - 1) / wgs;
   const int64_t most = mean / 256;
   n = n < most ? n : most;
   return static_cast<int>(n < 1 ? 1 : n > 256 ? 256 : n);
