@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
   constexpr bool kTwo = sizeof(T) == 2;  // V double-buffered too (fp32: LDS holds three tiles)
   constexpr bool kDma = VEC && kTwo;
-  std::conditional_t<kDma, TileDma<HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
+  std::conditional_t<kDma, TileDma<T, HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
   if constexpr (kDma) {
     tk.init(a.hd, [&](int r) { return r * a.ks; });
     tv.init(a.hd, [&](int r) { return r * a.vs; });
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kern
   // laid out alike; groups of more than 32 heads (not VEC) divide for every row.
   const int toks = VEC ? kBQ / a.group : 0, trows = VEC ? toks * a.group : kBQ;
   constexpr bool kDma = VEC && sizeof(T) == 2;
-  std::conditional_t<kDma, TileDma<HD, kBQ, kNT>, Tile<T, HD, kBQ, kNT, VEC>> tq, tg;
+  std::conditional_t<kDma, TileDma<T, HD, kBQ, kNT>, Tile<T, HD, kBQ, kNT, VEC>> tq, tg;
   const int64_t gs = static_cast<int64_t>(a.hq) * a.hd;
   const T* qbase = static_cast<const T*>(a.q) + sp.q0 * a.qs + int64_t(kvh) * a.group * a.hd;
   const T* gbase = dout + sp.q0 * gs + int64_t(kvh) * a.group * a.hd;

@@ -342,33 +342,33 @@ struct Tile {
   }
 };
 
-// The same tile straight from memory to LDS, 16 bytes a lane, without registers on the way
-// (bf16).  A wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in
+// The same tile straight from memory to LDS, 16 bytes a lane, without registers on the way.  A wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in
 // which chunk a lane reads.  A row at or past `rows` (of one stride each, or the last one of
 // row_off's) and channels at or past hd lie behind the buffer's end and arrive as zeros.
 // NT: threads that share a tile, a workgroup's or (64) one wave's.
-template <int HD, int ROWS, int NT>
+template <typename T, int HD, int ROWS, int NT>
 struct TileDma {
-  static constexpr int kChunks = HD / 8;
+  static constexpr int E = Elem<T>::kPerChunk;
+  static constexpr int kChunks = HD / E;
   static constexpr int kItems = (ROWS * kChunks + NT - 1) / NT;
   static_assert(ROWS * kChunks % 64 == 0, "whole waves");
   uint32_t voff[kItems];
 
-  // row_off(r): element offset of row r from the tile's first, below 2^30; negative: no row
+  // row_off(r): element offset of row r from the tile's first, below 2^29; negative: no row
   template <typename RowOff>
   __device__ __forceinline__ void init(int hd, RowOff row_off) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int item = static_cast<int>(threadIdx.x) % NT + i * NT;
       const int row = item / kChunks;
-      const int c = (item % kChunks ^ swz<bf16, HD>(row)) * 8;
+      const int c = (item % kChunks ^ swz<T, HD>(row)) * E;
       const int64_t off = row_off(row);
-      voff[i] = off < 0 || c >= hd ? 0x80000000u : static_cast<uint32_t>(off + c) * 2;
+      voff[i] = off < 0 || c >= hd ? 0x80000000u : static_cast<uint32_t>(off + c) * sizeof(T);
     }
   }
 
   // p: the tile's first row, the same in every lane; bytes: from p to the end of its last row
-  __device__ __forceinline__ void issue(const bf16* p, int64_t bytes, const bf16* lds) const {
+  __device__ __forceinline__ void issue(const T* p, int64_t bytes, const T* lds) const {
     const uint64_t at = reinterpret_cast<uint64_t>(p);
     const uint32_t n = bytes < 0 ? 0u : bytes > 0x7fffffff ? 0x7fffffffu : static_cast<uint32_t>(bytes);
     u32x4 rsrc = {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu, n,
@@ -376,12 +376,12 @@ struct TileDma {
 #pragma unroll
     for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
     const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) bf16*)lds)));
+        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) T*)lds)));
     const uint32_t wave =
         NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      if (ROWS * kChunks % NT != 0 && wave + i * NT * 16 >= ROWS * HD * 2) break;
+      if (ROWS * kChunks % NT != 0 && wave + i * NT * 16 >= ROWS * HD * sizeof(T)) break;
       // writes LDS only: no register is an output (nothing else here uses m0); waited for by
       // dma_wait
       asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"

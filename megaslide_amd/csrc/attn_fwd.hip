@@ -67,7 +67,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? (HD <= 64 ? 4 : 2) : 1) v
   const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
   // bf16 rows of 16-byte chunks go straight to LDS, others through registers
   constexpr bool kDma = VEC && sizeof(T) == 2;
-  std::conditional_t<kDma, TileDma<HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
+  std::conditional_t<kDma, TileDma<T, HD, kBN, kNT>, Tile<T, HD, kBN, kNT, VEC>> tk, tv;
   if constexpr (kDma) {
     tk.init(a.hd, [&](int r) { return r * a.ks; });
     tv.init(a.hd, [&](int r) { return r * a.vs; });
@@ -230,31 +230,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
   if (lse != nullptr && lane == 0) lse[row] = sum == 0.0f ? -INFINITY : base + logf(sum);
 }
 
-// One new token each over caches (bf16): as many workgroups a sequence and key head as it has
+// One new token each over caches: as many workgroups a sequence and key head as it has
 // chunks of keys, so that long and short caches share the device evenly.  Bound: memory, K and V
-// once.  The group's heads are the rows of one block; the four waves take every fourth tile of
-// 32 keys of the chunk for themselves and meet only at its end, so no wave waits for another.
+// once.  The group's heads are the rows of one block; the NW waves take every NW-th tile of 32
+// keys of the chunk for themselves and meet only at its end, so no wave waits for another.
 // A wave's next keys are on their way to LDS while it weighs the present values, and the next
 // values while it scores the next keys.  Parts are joined by attn_join_tokens_kernel.
 // 134,000 keys of 16 sequences, 32/8 heads x 128: 114 us, 4.8 TB/s (a copy reaches 5.1).
-template <int HD>
-__global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
-                                                             bf16* __restrict__ out,
-                                                             bf16* __restrict__ rest,
-                                                             float* __restrict__ lse,
-                                                             float* __restrict__ part, int chunk,
-                                                             int64_t units) {
-  constexpr int kKK = HD / 16, kBlk = HD / 32, kN = 32;
-  constexpr int kLoads = TileDma<HD, kN, 64>::kItems;
+template <typename T, int HD>
+constexpr int kTokenWaves = sizeof(T) == 4 && HD > 64 ? 2 : 4;  // their tiles fill 64 KB of LDS
+
+template <typename T, int HD>
+__global__ __launch_bounds__((kTokenWaves<T, HD> * 64), sizeof(T) == 4 ? 1 : 2)
+void attn_tokens_kernel(const AttnArgs a, T* __restrict__ out, T* __restrict__ rest,
+                        float* __restrict__ lse, float* __restrict__ part, int chunk,
+                        int64_t units) {
+  typedef typename Elem<T>::frag Frag;
+  constexpr int kKK = HD / 16, kBlk = HD / 32, kN = 32, NW = kTokenWaves<T, HD>;
+  constexpr int kLoads = TileDma<T, HD, kN, 64>::kItems;
   // the tiles that loads fill directly come first: such loads reach 64 KB of LDS
   __shared__ struct {
     union {
       struct {
-        alignas(16) bf16 k[kN * HD], v[kN * HD];
-      } w[4];
-      float o[4][32][HD];
+        alignas(16) T k[kN * HD], v[kN * HD];
+      } w[NW];
+      float o[NW][32][HD];
     };
-    float m[4][32], l[4][32];
+    float m[NW][32], l[NW][32];
   } sm;
 
   const int slot = blockIdx.x / static_cast<unsigned>(a.hk);
@@ -267,11 +269,11 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
   const int64_t kbase = a.cu_k == nullptr ? static_cast<int64_t>(sp.seq) * a.nk
                                           : bound_of(a.cu_k, sp.seq, a.total_k);
   const int64_t unit = kbase / chunk + sp.seq + sp.tile;
-  const bf16* kp = static_cast<const bf16*>(a.k) + sp.k0 * a.ks + int64_t(kvh) * a.hd;
-  const bf16* vp = static_cast<const bf16*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
-  bf16* const sk = sm.w[wave].k;
-  bf16* const sv = sm.w[wave].v;
-  TileDma<HD, kN, 64> tk, tv;
+  const T* kp = static_cast<const T*>(a.k) + sp.k0 * a.ks + int64_t(kvh) * a.hd;
+  const T* vp = static_cast<const T*>(a.v) + sp.k0 * a.vs + int64_t(kvh) * a.hd;
+  T* const sk = sm.w[wave].k;
+  T* const sv = sm.w[wave].v;
+  TileDma<T, HD, kN, 64> tk, tv;
   tk.init(a.hd, [&](int r) { return r * a.ks; });
   tv.init(a.hd, [&](int r) { return r * a.vs; });
   const float c = a.scale * kLog2e;
@@ -288,35 +290,35 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
     const int from = tok == 0 ? sp.tile * chunk : 0;
     int to = tok == 0 && from + chunk < limit ? from + chunk : limit;
     to = to < from ? from : to;
-    const bf16* qp = static_cast<const bf16*>(a.q) + (sp.q0 + tok) * a.qs + int64_t(head) * a.hd;
-    bf16x8 q[kKK];
+    const T* qp = static_cast<const T*>(a.q) + (sp.q0 + tok) * a.qs + int64_t(head) * a.hd;
+    Frag q[kKK];
 #pragma unroll
-    for (int i = 0; i < kKK; ++i) q[i] = mem_frag<bf16, true>(qp, i * 16 + g * 8, a.hd);
+    for (int i = 0; i < kKK; ++i) q[i] = mem_frag<T, true>(qp, i * 16 + g * 8, a.hd);
     f32x16 o[kBlk];
 #pragma unroll
     for (int b = 0; b < kBlk; ++b) o[b] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     const auto load_k = [&](int k0) __attribute__((always_inline)) {
-      tk.issue(kp + k0 * a.ks, (sp.lk - k0) * a.ks * 2, sk);
+      tk.issue(kp + k0 * a.ks, (sp.lk - k0) * a.ks * int64_t(sizeof(T)), sk);
     };
     const auto load_v = [&](int k0) __attribute__((always_inline)) {
-      tv.issue(vp + k0 * a.vs, (sp.lk - k0) * a.vs * 2, sv);
+      tv.issue(vp + k0 * a.vs, (sp.lk - k0) * a.vs * int64_t(sizeof(T)), sv);
     };
     int64_t k0 = from + wave * kN;
     if (k0 < to) {
       load_k(k0);
       load_v(k0);
     }
-    for (; k0 < to; k0 += 4 * kN) {
+    for (; k0 < to; k0 += NW * kN) {
       dma_wait<kLoads>();  // the keys
       f32x16 s = {};
 #pragma unroll
       for (int i = 0; i < kKK; ++i)
-        s = mma(row_frag<bf16, HD>(sk, lane & 31, i * 16 + g * 8), q[i], s);
-      const bool more = k0 + 4 * kN < to;
+        s = mma(row_frag<T, HD>(sk, lane & 31, i * 16 + g * 8), q[i], s);
+      const bool more = k0 + NW * kN < to;
       // (all reads of the tile are back before it is overwritten)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) load_k(k0 + 4 * kN);
+      if (more) load_k(k0 + NW * kN);
       if (k0 + kN > to) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -346,10 +348,10 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
         dma_wait();
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
-        const bf16x8 p = to_frag<bf16>(s, t2);
+        const Frag p = to_frag<T>(s, t2);
 #pragma unroll
         for (int d = 0; d < kBlk; ++d) {
-          bf16x8 v = col_frag<bf16, HD>(sv, t2 * 16, d);
+          Frag v = col_frag<T, HD>(sv, t2 * 16, d);
           // keys behind the limit have weight zero, and their values may not be finite
           if (k0 + kN > to) {
 #pragma unroll
@@ -360,11 +362,11 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) load_v(k0 + 4 * kN);
+      if (more) load_v(k0 + NW * kN);
     }
     l = half_sum(l);
 
-    // the four waves' parts, of the group's rows
+    // the waves' parts, of the group's rows
     __syncthreads();
     if ((lane & 31) < a.group) {
 #pragma unroll
@@ -379,14 +381,14 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < a.group * HD; i += 256) {
+    for (int i = threadIdx.x; i < a.group * HD; i += NW * 64) {
       const int row = i / HD, ch = i - row * HD;
       float top = -INFINITY, acc = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sm.m[w][row]);
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, sm.m[w][row]);
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = exp2f((sm.m[w][row] - base) * c);
         acc += f * sm.o[w][row][ch];
         sum += f * sm.l[w][row];
@@ -399,9 +401,9 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
         if (ch == 0) part[units * a.hq * HD + r] = ls;
       } else {
         const int64_t r = (sp.q0 + tok) * a.hq + kvh * a.group + row;
-        if (ch < a.hd) out[r * a.hd + ch] = from_f32<bf16>(acc);
+        if (ch < a.hd) out[r * a.hd + ch] = from_f32<T>(acc);
         if (ch < a.hd && rest != nullptr)
-          rest[r * a.hd + ch] = from_f32<bf16>(rest_of<bf16>(acc));
+          rest[r * a.hd + ch] = from_f32<T>(rest_of<T>(acc));
         if (ch == 0 && lse != nullptr) lse[r] = ls;
       }
     }
@@ -412,9 +414,10 @@ __global__ __launch_bounds__(256, 2) void attn_tokens_kernel(const AttnArgs a,
 // Joins the chunks of every sequence's first token, one workgroup a (row, head), its waves every
 // fourth chunk each; rows that no key belongs to (behind the last sequence, or of a sequence
 // without keys) become 0 and -inf.
+template <typename T>
 __global__ __launch_bounds__(256) void attn_join_tokens_kernel(
     const AttnArgs a, const float* __restrict__ part, int chunk, int64_t units, int hd_padded,
-    bf16* __restrict__ out, bf16* __restrict__ rest, float* __restrict__ lse) {
+    T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse) {
   __shared__ float s_acc[4][128], s_sum[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.x / static_cast<unsigned>(a.hq);
@@ -463,8 +466,8 @@ __global__ __launch_bounds__(256) void attn_join_tokens_kernel(
   if (ch < a.hd) {
     float v = s_acc[0][ch] + s_acc[1][ch] + s_acc[2][ch] + s_acc[3][ch];
     v = sum == 0.0f ? 0.0f : v / sum;
-    out[r * a.hd + ch] = from_f32<bf16>(v);
-    if (rest != nullptr) rest[r * a.hd + ch] = from_f32<bf16>(rest_of<bf16>(v));
+    out[r * a.hd + ch] = from_f32<T>(v);
+    if (rest != nullptr) rest[r * a.hd + ch] = from_f32<T>(rest_of<T>(v));
   }
   if (lse != nullptr && ch == 0) lse[r] = sum == 0.0f ? -INFINITY : base + logf(sum);
 }
@@ -499,8 +502,7 @@ constexpr int kNW = 4;
 // right too, and slower); a group is the rows of one block; below 1,024 keys in all the kernel
 // that needs no joining is faster.
 int token_chunk(const msd_attn_desc& d) {
-  if (d.dtype != MSD_BF16 || d.total_q != d.num_seqs || d.num_heads / d.num_kv_heads > 32 ||
-      d.total_k < 1024)
+  if (d.total_q != d.num_seqs || d.num_heads / d.num_kv_heads > 32 || d.total_k < 1024)
     return 0;
   const int64_t n = (d.total_k * d.num_kv_heads / 2048 + 127) / 128 * 128;
   return static_cast<int>(n < 256 ? 256 : n > 2048 ? 2048 : n);
@@ -510,17 +512,18 @@ int64_t token_units(const msd_attn_desc& d, int chunk) {
   return d.total_k / chunk + d.num_seqs + 1;
 }
 
-template <int HD>
-hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, bf16* out, bf16* rest,
-                         float* lse, float* ws, int chunk, hipStream_t s) {
+template <typename T, int HD>
+hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, T* out, T* rest, float* lse,
+                         float* ws, int chunk, hipStream_t s) {
   const int64_t units = token_units(d, chunk);
   int64_t slots = units;
   if (a.cu_q == nullptr) slots = (d.total_k / d.num_seqs + chunk - 1) / chunk * d.num_seqs;
-  attn_tokens_kernel<HD><<<static_cast<unsigned>(slots * a.hk), 256, 0, s>>>(
-      a, out, rest, lse, ws, chunk, units);
+  attn_tokens_kernel<T, HD>
+      <<<static_cast<unsigned>(slots * a.hk), kTokenWaves<T, HD> * 64, 0, s>>>(
+          a, out, rest, lse, ws, chunk, units);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  attn_join_tokens_kernel<<<static_cast<unsigned>(a.total_q * a.hq), 256, 0, s>>>(
+  attn_join_tokens_kernel<T><<<static_cast<unsigned>(a.total_q * a.hq), 256, 0, s>>>(
       a, ws, chunk, units, HD, out, rest, lse);
   return hipGetLastError();
 }
@@ -528,10 +531,8 @@ hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, bf16* out, b
 template <typename T, int HD>
 hipError_t launch_hd(const msd_attn_desc& d, const AttnArgs& a, T* out, T* rest, float* lse,
                      float* ws, bool vec, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    const int chunk = vec ? token_chunk(d) : 0;
-    if (chunk > 0) return launch_tokens<HD>(d, a, out, rest, lse, ws, chunk, s);
-  }
+  const int chunk = vec ? token_chunk(d) : 0;
+  if (chunk > 0) return launch_tokens<T, HD>(d, a, out, rest, lse, ws, chunk, s);
   const bool packed = a.cu_q != nullptr;
   const int n = splits(d, packed, kNW * 32);
   const int64_t slots = q_slots(d, packed, kNW * 32);
@@ -598,10 +599,10 @@ bool attn_vec(const msd_attn_desc& d, const AttnArgs& a, bool bwd) {
   const int64_t e = d.dtype == MSD_BF16 ? 2 : 4;
   const auto ok = [&](const void* p, int64_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * e % 16 == 0 &&
-           stride <= (int64_t(1) << 23);  // a tile's rows are 32-bit offsets
+           stride <= (int64_t(1) << 22);  // a tile's rows are 32-bit offsets
   };
   return a.hd % 8 == 0 && ok(a.q, a.qs) && ok(a.k, a.ks) && ok(a.v, a.vs) &&
-         (!bwd || (a.group <= 32 && int64_t(a.hq) * a.hd <= (int64_t(1) << 23)));
+         (!bwd || (a.group <= 32 && int64_t(a.hq) * a.hd <= (int64_t(1) << 22)));
 }
 
 // Upper bound over both forms (packed or equal lengths): the descriptor does not say which.

@@ -193,28 +193,42 @@ class _RopeCall:
 class AxialRopeFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, call):
-        ctx.call = call
-        ctx.dtype = x.dtype
-        return call.forward(x, None)[0]
+        y = call.forward(x, None)[0]
+        ctx.call, ctx.dtype = call, x.dtype
+        ctx.save_for_backward(call.pos)
+        call.pos = None
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return ctx.call.backward(None, None, dy.to(ctx.dtype), None, (False, False))[0], None
+        call = ctx.call
+        (call.pos,) = ctx.saved_tensors
+        try:
+            return call.backward(None, None, dy.to(ctx.dtype), None, (False, False))[0], None
+        finally:
+            call.pos = None
 
 
 class QkNormRopeFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, call):
+        ys = call.forward(q, k)
         ctx.call = call
-        ctx.save_for_backward(q, k)
-        return call.forward(q, k)
+        ctx.save_for_backward(q, k, *call.weights, call.pos)
+        call.weights = call.pos = None
+        return ys
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dyq, dyk):
-        q, k = ctx.saved_tensors
-        return (*ctx.call.backward(q, k, dyq.to(q.dtype), dyk, ctx.needs_input_grad[2:4]), None)
+        call = ctx.call
+        q, k, wq, wk, call.pos = ctx.saved_tensors
+        call.weights = (wq, wk)
+        try:
+            return (*call.backward(q, k, dyq.to(q.dtype), dyk, ctx.needs_input_grad[2:4]), None)
+        finally:
+            call.weights = call.pos = None
 
 
 def axial_rope(x: Tensor, positions: Positions, num_heads: int,
@@ -315,6 +329,15 @@ class _AttnCall:
             num_kv_heads, hd, _lib.dtype_code(dt), 1 if causal else 0,
             1.0 / math.sqrt(hd) if scale is None else float(scale))
 
+    def take(self):
+        """The call's tensors, which it then holds no more (autograd saves them)."""
+        tensors = (self.q, self.k, self.v, self.cu_q, self.cu_k)
+        self.q = self.k = self.v = self.cu_q = self.cu_k = None
+        return tensors
+
+    def give(self, tensors) -> None:
+        self.q, self.k, self.v, self.cu_q, self.cu_k = tensors
+
     def forward(self, want_lse: bool, want_rest: bool = False):
         """out, lse and what rounding took from out (bf16, for the backward), as wanted."""
         q, ptr = self.q, _lib.ptr
@@ -399,6 +422,33 @@ def _attn_backward(ctx, dout, dlse, drest):
 _attn_fwd_op.register_autograd(_attn_backward, setup_context=_attn_setup)
 
 
+class PackedAttentionFunction(torch.autograd.Function):
+    """The custom operator's forward and backward without the dispatcher between, which would
+    cost a small training call several times its kernels' time; for calls that no dispatch mode
+    (selective checkpointing) and no compiler has to see."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, call):
+        out, lse, rest = call.forward(want_lse=True, want_rest=True)
+        ctx.call = call
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*call.take(), out, lse, rest)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlse):
+        *tensors, out, lse, rest = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(out)
+        call = ctx.call
+        call.give(tensors)
+        try:
+            return (*call.backward(out, lse, rest, dout, dlse), None)
+        finally:
+            call.take()
+
+
 def packed_attention(q: Tensor, k: Tensor, v: Tensor, num_heads: int,
                      num_kv_heads: Optional[int] = None, cu_seqlens: Optional[Tensor] = None,
                      cu_seqlens_k: Optional[Tensor] = None, causal: bool = False,
@@ -423,7 +473,11 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, num_heads: int,
     """
     num_heads = int(num_heads)
     num_kv_heads = int(num_heads if num_kv_heads is None else num_kv_heads)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0:
+            out, lse = PackedAttentionFunction.apply(q, k, v, _AttnCall(
+                q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, causal, scale))
+            return (out, lse) if return_lse else out
         out, lse, _ = torch.ops.megaslide.packed_attention(
             q, k, v, cu_seqlens, cu_seqlens_k, num_heads, num_kv_heads, bool(causal),
             None if scale is None else float(scale))
