@@ -246,6 +246,77 @@ def test_rows_behind_the_last_sequence(dt):
         assert torch.equal(a[80:], torch.full_like(a[80:], fill))
 
 
+@pytest.mark.parametrize("S", [3, 63, 64, 100])
+def test_rows_behind_many_sequences(S):
+    """The same with more sequences than a wave has lanes, and as many tokens as sequences."""
+    from megaslide_amd import packed_attention
+    g = gen(S)
+    for lq, lk in (([(i * 5) % 9 for i in range(S)], [(i * 5) % 9 for i in range(S)]),
+                   ([1] * (S - 1) + [0], [(i * 31) % 77 for i in range(S)])):
+        n, m = sum(lq), sum(lk)
+        extra = 1 if lq[-1] == 0 and sum(lq) == S - 1 else 37
+        q = randn(g, n + extra, 64, dt=BF)
+        k, v = randn(g, m + 50, 32, dt=BF), randn(g, m + 50, 32, dt=BF)
+        q[n:], k[m:], v[m:] = math.nan, math.nan, math.nan
+        ins = [t.requires_grad_(True) for t in (q, k, v)]
+        out = packed_attention(q, k, v, 2, 1, lens_to_cu(lq, DEV), lens_to_cu(lk, DEV), True)
+        dout = randn(g, n + extra, 64, dt=BF)
+        grads = torch.autograd.grad(out, ins, dout)
+        with torch.no_grad():
+            want, err = attention(q[:n], k[:m], v[:m], lq, lk, 2, 1, True, dout=dout[:n])
+            for a, b, e, r in zip((out, *grads), (want[0], *want[2:]), (err[0], *err[2:]),
+                                  (n, n, m, m)):
+                assert_within(a[:r], b, e, "rows")
+                assert not a[r:].any()
+
+
+def test_strides_and_offsets_beyond_32_bits():
+    """Keys and values whose rows lie further apart than a tile's 32-bit offsets reach, and whose
+    last rows lie beyond 2^32 bytes and elements of the first: the bits of contiguous ones."""
+    from megaslide_amd import packed_attention
+    g = gen(21)
+    heads, kv, hd = 4, 2, 64
+    for n, stride in ((2100, 1 << 21), (9, (1 << 22) + 8)):
+        print(f"[attn] {n} rows {stride} apart", flush=True)
+        k, v = randn(g, n, kv * hd, dt=BF), randn(g, n, kv * hd, dt=BF)
+        q = randn(g, n, heads * hd, dt=BF)
+        big = torch.empty(n * stride, dtype=BF, device=DEV).view(n, stride)
+        kb, vb = big[:, :kv * hd], big[:, 512:512 + kv * hd]
+        kb.copy_(k)
+        vb.copy_(v)
+
+        def call(q, k, v):
+            ins = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = packed_attention(*ins, heads, kv, causal=True)
+            return [out.detach(), *torch.autograd.grad(out, ins, q)]
+
+        assert all(torch.equal(a, b) for a, b in zip(call(q, kb, vb), call(q, k, v)))
+        cu = lens_to_cu([1], DEV), lens_to_cu([n], DEV)  # one token over the cache
+        assert torch.equal(packed_attention(q[:1], kb, vb, heads, kv, *cu),
+                           packed_attention(q[:1], k, v, heads, kv, *cu))
+        del big, kb, vb
+
+
+def test_saved_tensors():
+    """A backward that is run twice, and one after its inputs were written to (an error)."""
+    from megaslide_amd import packed_attention, qk_norm_rope
+    q, k, v, dout = inputs([40], [40], 2, 2, 32, BF)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = packed_attention(q, k, v, 2, causal=True)
+    a = torch.autograd.grad(out, (q, k, v), dout, retain_graph=True)
+    b = torch.autograd.grad(out, (q, k, v), dout)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    pos = torch.arange(40, device=DEV)[:, None]
+    w = torch.ones(32, device=DEV)
+    for change in (lambda: v.detach().mul_(2), lambda: pos.add_(1), lambda: w.add_(1)):
+        qr, kr = qk_norm_rope(q, k, w, w, pos, 2)
+        out = packed_attention(qr, kr, v, 2, causal=True)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, (q, k, v), dout)
+
+
 @pytest.mark.parametrize("dt", [BF, F32])
 @pytest.mark.parametrize("hd", [32, 128])
 def test_nonfinite_values_stay_where_they_are_seen(dt, hd):
