@@ -336,7 +336,12 @@ class _AttnCall:
         return tensors
 
     def give(self, tensors) -> None:
-        self.q, self.k, self.v, self.cu_q, self.cu_k = tensors
+        """Those tensors again, whose layout may be another one (hooks on saved tensors move and
+        copy them)."""
+        q, k, v, self.cu_q, self.cu_k = tensors
+        self.q, self.desc.q_stride = _rows(q, "q")
+        self.k, self.desc.k_stride = _rows(k, "k")
+        self.v, self.desc.v_stride = _rows(v, "v")
 
     def forward(self, want_lse: bool, want_rest: bool = False):
         """out, lse and what rounding took from out (bf16, for the backward), as wanted."""

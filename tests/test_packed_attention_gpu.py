@@ -455,6 +455,25 @@ def test_empty_calls():
     assert packed_attention(b, b, b, 4).shape == b.shape
 
 
+def test_saved_tensors_of_another_layout():
+    """Hooks on saved tensors hand back contiguous copies of the views that were saved."""
+    from megaslide_amd import packed_attention
+    g = gen(9)
+    qkv = randn(g, 150, 8 * 64, dt=BF).requires_grad_(True)
+    cu = lens_to_cu([70, 80], DEV)
+
+    def f():
+        q, k, v = qkv.split([256, 128, 128], -1)
+        return packed_attention(q, k, v, 4, 2, cu, causal=True)
+
+    dout = randn(g, 150, 256, dt=BF)
+    (want,) = torch.autograd.grad(f(), qkv, dout)
+    with torch.autograd.graph.save_on_cpu():
+        out = f()
+    (got,) = torch.autograd.grad(out, qkv, dout)
+    assert torch.equal(got, want)
+
+
 def test_checkpoint_keeps_the_attention():
     """The selective policy that keeps the deformable core's outputs keeps this one's too."""
     from torch.utils.checkpoint import checkpoint
