@@ -114,9 +114,11 @@ int check_qk_rope(const msd_qk_rope_desc* d) {
   if (d->n_axes < 1 || d->n_axes > 4)
     return fail(MSD_ERR_ARG, "qk_rope: %d axes outside [1, 4]", d->n_axes);
   if (d->pos_dtype == MSD_POS_GRID &&
-      (d->n_axes != 3 || d->grid[0] < 1 || d->grid[1] < 1 || d->grid[2] < 1 ||
-       d->pos_rows / d->grid[0] / d->grid[1] != d->grid[2] ||
-       d->pos_rows % d->grid[0] != 0 || d->pos_rows / d->grid[0] % d->grid[1] != 0))
+      (d->n_axes != 3 ||
+       (d->tokens > 0 && (d->grid[0] < 1 || d->grid[1] < 1 || d->grid[2] < 1 ||
+                          d->pos_rows / d->grid[0] / d->grid[1] != d->grid[2] ||
+                          d->pos_rows % d->grid[0] != 0 ||
+                          d->pos_rows / d->grid[0] % d->grid[1] != 0))))
     return fail(MSD_ERR_ARG, "qk_rope: grid (%d, %d, %d) needs 3 axes and as many position rows",
                 d->grid[0], d->grid[1], d->grid[2]);
   int64_t sum = 0;
@@ -153,9 +155,11 @@ int check_attn(const msd_attn_desc* d) {
     return fail(MSD_ERR_UNSUPPORTED, "attn: dtype %d not supported", d->dtype);
   if (d->causal != 0 && d->causal != 1) return fail(MSD_ERR_ARG, "attn: causal %d", d->causal);
   if (d->num_seqs < 1) return fail(MSD_ERR_ARG, "attn: num_seqs=%d", d->num_seqs);
-  // row and workgroup counts are 32-bit
+  // rows are counted in 32 bits; a launch has below 2^24 workgroups of 256 threads: one for each
+  // 128 rows and one a sequence and head
   constexpr int64_t kMost = int64_t(1) << 30;
-  if (d->total_q < 0 || d->total_k < 0 || d->num_heads > 65536 || d->num_seqs > kMost / d->num_heads ||
+  if (d->total_q < 0 || d->total_k < 0 || d->num_heads > 65536 ||
+      d->num_seqs > (kMost >> 8) / d->num_heads ||
       d->total_q > kMost / d->num_heads || d->total_k > kMost / d->num_kv_heads)
     return fail(MSD_ERR_ARG, "attn: sizes out of range (total_q=%lld, total_k=%lld, num_seqs=%d)",
                 (long long)d->total_q, (long long)d->total_k, d->num_seqs);
@@ -440,6 +444,8 @@ int msd_qk_rope_bwd(const msd_qk_rope_desc* desc, const void* q, const void* k,
                         static_cast<const void*>(dk_weight)})
     if (p != nullptr && !aligned(p, elem_bytes(desc->weight_dtype)))
       return fail(MSD_ERR_ALIGN, "qk_rope_bwd: weight misaligned");
+  if (dk_weight != nullptr && desc->k_heads == 0)
+    return fail(MSD_ERR_ARG, "qk_rope_bwd: dk_weight without k");
   const size_t need = msd::qk_rope_bwd_ws_bytes(*desc);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(MSD_ERR_WORKSPACE,

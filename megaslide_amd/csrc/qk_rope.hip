@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kThreads, 4) void qk_rope_kernel(const RopeArgs a) 
     int at = 0;
     for (int x = 0; x < a.n_axes; ++x) {
       const int d = a.axis[x], l = c - at;
-      if (l >= 0 && l < d) {
+      if (l >= 0 && l < d && grp < kRows) {  // (an idle lane stays within its own slot of s_row)
         const int half = d / 2;
         // axes are even and begin at even channels, so c ^ 1 is within the axis
         const bool second = INTER ? (l & 1) : l >= half;

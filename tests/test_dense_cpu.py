@@ -79,6 +79,24 @@ def test_rope_pointers_and_workspace():
     assert lib.msd_qk_rope_bwd_workspace_size(None) == 0
 
 
+def test_rope_keyless_and_empty_calls():
+    """A gradient of a weight that no key has is refused; no tokens need no grid."""
+    lib = _lib.load()
+    d = rope_desc(k_heads=0)
+    assert lib.msd_qk_rope_bwd(ctypes.byref(d), *([16] * 11), 16, 1 << 30, None) == -1
+    assert b"dk_weight" in lib.msd_last_error()
+    assert rope_fwd(rope_desc(tokens=0, pos_rows=0, pos_dtype=4), (None,) * 7) == 0
+
+
+def test_attention_sequence_limit():
+    """More sequences than a launch has workgroups for are refused, as many as fit are not."""
+    lib = _lib.load()
+    at = attn_desc(num_seqs=1 << 20, total_q=0)
+    assert attn_fwd(at, q=None, out=None) == 0
+    assert attn_fwd(attn_desc(num_seqs=(1 << 20) + 1, total_q=0)) == -1
+    assert b"range" in lib.msd_last_error()
+
+
 def attn_desc(**kw):
     d = dict(total_q=24, total_k=40, q_stride=256, k_stride=128, v_stride=128, num_seqs=2,
              num_heads=4, num_kv_heads=2, head_dim=64, dtype=1, causal=1, scale=0.125)

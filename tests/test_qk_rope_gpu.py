@@ -217,6 +217,27 @@ def test_empty_and_nonfinite():
     assert torch.equal(yz, torch.zeros_like(yz)) and torch.isfinite(dz).all()
 
 
+def test_saved_tensors_of_another_layout():
+    """Hooks on saved tensors hand back contiguous copies of the views that were saved."""
+    from megaslide_amd import qk_norm_rope
+    g = gen(10)
+    qkv = randn(g, 60, 6 * 64, dt=BF).requires_grad_(True)
+    w = [randn(g, 64).requires_grad_(True) for _ in range(2)]
+    dq, dk = randn(g, 60, 128, dt=BF), randn(g, 60, 128, dt=BF)
+
+    def f():
+        q, k, _ = qkv.split(128, -1)
+        return qk_norm_rope(q, k, *w, (3, 4, 5), 2)
+
+    want = torch.autograd.grad(f(), (qkv, *w), (dq, dk))
+    with torch.autograd.graph.save_on_cpu():
+        out = f()
+    got = torch.autograd.grad(out, (qkv, *w), (dq, dk))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    empty = qkv[:0, :128]
+    assert qk_norm_rope(empty, empty, None, None, (0, 4, 5), 2)[0].shape == (0, 128)
+
+
 def test_streams_and_graph():
     """On a side stream, and captured with its backward and replayed on new contents."""
     from megaslide_amd import qk_norm_rope
