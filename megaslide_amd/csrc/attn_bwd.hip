@@ -235,8 +235,8 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kern
   for (int i = 0; i < kKK; ++i) {
     kf[i] = mem_frag<T, VEC>(kp, i * 16 + g * 8, a.hd);
     const Frag v = mem_frag<T, VEC>(vp, i * 16 + g * 8, a.hd);
-    if constexpr (kWide)  // (read by this wave only)
-      *reinterpret_cast<Frag*>(s_v + at<T, HD>(wave * 32 + (lane & 31), i * 16 + g * 8)) = v;
+    if constexpr (kWide)  // in the order in which this very lane reads it: one address for all
+      *reinterpret_cast<Frag*>(s_v + ((wave * kKK + i) * 64 + lane) * 8) = v;
     else
       vf[i] = v;
   }
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kern
           s = mma(row_frag<T, HD>(s_q[buf], b * 32 + (lane & 31), i * 16 + g * 8), kf[i], s);
           Frag v;
           if constexpr (kWide)
-            v = row_frag<T, HD>(s_v, wave * 32 + (lane & 31), i * 16 + g * 8);
+            v = *reinterpret_cast<const Frag*>(s_v + ((wave * kKK + i) * 64 + lane) * 8);
           else
             v = vf[i];
           dp = mma(row_frag<T, HD>(s_g[buf], b * 32 + (lane & 31), i * 16 + g * 8), v, dp);
