@@ -342,10 +342,11 @@ struct Tile {
   }
 };
 
-// The same tile straight from memory to LDS, 16 bytes a lane, without registers on the way.  A wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in
-// which chunk a lane reads.  A row at or past `rows` (of one stride each, or the last one of
-// row_off's) and channels at or past hd lie behind the buffer's end and arrive as zeros.
-// NT: threads that share a tile, a workgroup's or (64) one wave's.
+// The same tile straight from memory to LDS, 16 bytes a lane, without registers on the way.  A
+// wave's lanes fill 1,024 bytes of LDS in lane order; the XOR of the chunks is in which chunk a lane
+// reads.  A row at or past `rows` (of one stride each, or the last one of row_off's) and channels
+// at or past hd lie behind the buffer's end and arrive as zeros.  NT: threads that share a tile, a
+// workgroup's or (64) one wave's.
 template <typename T, int HD, int ROWS, int NT>
 struct TileDma {
   static constexpr int E = Elem<T>::kPerChunk;

@@ -7,6 +7,18 @@
 // rows along the lanes, so that m, l and the rescale of O are one value a lane and P is a
 // fragment where it stands.  m is raised only where a score exceeds it by 2^8 or more in p
 // (p <= 256: nothing is lost in fp32), which spares most rescales.
+//
+// Bound: the matrix cores and the vector unit one after the other.  Of the cycles of a SIMD the
+// products take 45 % and the vector instructions 50 % (8,192 tokens, 16 x 64, bf16; 41 % and 35 %
+// at 16/4 heads x 128, causal), two to four waves a SIMD notwithstanding; LDS is busy for 20 %, and
+// nine in ten requests hit the L2.  Four waves of 32 rows and 64 keys: eight waves, or 32 keys,
+// were 7 to 10 % slower, and so was the forward without the search for the maximum on the small
+// head sizes.  Tiles that a causal mask cuts are a loop of their own, so that the others compare
+// nothing.
+// Measured: 8,192 tokens, 16 x 64, bf16: 308 us, 890 TFLOP/s (a library product of that type
+// 1,300 to 1,570); packed sequences of 129 to 5,003 tokens, causal, 16/4 x 128: 239 us, 870; prompts
+// of 1 to 4,096, causal, 32/8 x 128: 233 us, 820; two fp32 clips of 2,048, 4 x 64: 96 us,
+// 90 TFLOP/s (a library product 153).
 #include "attn_common.h"
 
 namespace msd {

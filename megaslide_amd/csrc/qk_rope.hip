@@ -17,6 +17,9 @@
 // the lane's own chunk (interleaved pairs) or read through LDS (pairs half an axis apart, which
 // no fixed shuffle serves for odd splits).  Where tokens are few, their heads are split among
 // workgroups.
+// Measured (a copy reaches 5.1 TB/s): rotation of 46,800 tokens, 16 x 96, bf16, 68 us forward and
+// 68 backward, 4.2 TB/s; with the norm, 65,536 tokens, 16 + 16 heads x 64, bf16, 131 and 190 us, 4.1
+// and 4.2 TB/s; 32,768 tokens, 8 + 8 x 64, fp32, 64 and 83 us, 4.2 and 4.8 TB/s; 16 tokens 6 us.
 #include "common.h"
 #include "qk_rope.h"
 
@@ -188,7 +191,8 @@ __global__ __launch_bounds__(kThreads, 4) void qk_rope_kernel(const RopeArgs a) 
     int at = 0;
     for (int x = 0; x < a.n_axes; ++x) {
       const int d = a.axis[x], l = c - at;
-      if (l >= 0 && l < d && grp < kRows) {  // (an idle lane stays within its own slot of s_row)
+      // (an idle lane stays within its own slot of s_row)
+      if (l >= 0 && l < d && (64 % LPR == 0 || grp < kRows)) {
         const int half = d / 2;
         // axes are even and begin at even channels, so c ^ 1 is within the axis
         const bool second = INTER ? (l & 1) : l >= half;

@@ -470,9 +470,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, num_heads: int,
     Query head h reads key head h // (num_heads // num_kv_heads).  ``causal``: query i of n sees
     the keys j <= i + m - n (the last query sees the last key, so that one new token over a
     cache sees all of it).  A query that sees no key (or none with a score above -inf) has out 0 and
-    lse -inf.  What a query does
-    not see does not change its result, infinities and NaN there included.  ``scale``: default
-    1 / sqrt(head_dim); positive.  head_dim up to 128.
+    lse -inf.  What a query does not see does not change its result, infinities and NaN there
+    included.  ``scale``: default 1 / sqrt(head_dim); positive.  head_dim up to 128.
 
     Returns out like q (and lse, the log-sum-exp of the scaled scores, fp32 [..., num_heads]);
     both are differentiable, once.  Gradients are summed without atomics, in a fixed order.
