@@ -90,7 +90,10 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
   if (dlse != nullptr) delta -= dlse[at_row];
   float ls = lse[at_row];
   ls = ls == -INFINITY ? INFINITY : ls * kLog2e;  // a row without keys has no weights
-  if (mine && g == 0 && split == 0) stats[at_row] = make_float2(ls, delta);
+  if (mine && g == 0 && split == 0) stats[at_row] = make_float2(ls, -delta);
+  f32x16 minus;  // dO V^T - delta: the sum begins with it
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus[r] = -delta;
 
   f32x16 acc[kBlk];
 #pragma unroll
@@ -143,7 +146,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
     if (row0 < rows && (!kMasked || k0 < top)) {
 #pragma unroll
       for (int b = 0; b < kBN / 32; ++b) {
-        f32x16 s = {}, dp = {};
+        f32x16 s = {}, dp = minus;
 #pragma unroll
         for (int i = 0; i < kKK; ++i) {
           s = mma(row_frag<T, HD>(s_k[buf], b * 32 + (lane & 31), i * 16 + g * 8), q[i], s);
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dq_kerne
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[r] = __builtin_amdgcn_exp2f(s[r] * c - ls) * (dp[r] - delta);
+          s[r] = __builtin_amdgcn_exp2f(s[r] * c - ls) * dp[r];
           if (kMasked && k0 + b * 32 + 8 * (r / 4) + 4 * g + r % 4 >= limit) s[r] = 0.0f;
         }
 #pragma unroll
@@ -345,7 +348,13 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kern
       for (int b = 0; b < kBQ / 32; ++b) {
         const int r0 = t * trows + b * 32;
         if (kMasked && r0 + 32 <= wfirst) continue;
-        f32x16 s = {}, dp = {};
+        f32x16 s = {}, dp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 de = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + 8 * i + 4 * g]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dp[4 * i + j] = de[j];
+        }
 #pragma unroll
         for (int i = 0; i < kKK; ++i) {
           s = mma(row_frag<T, HD>(s_q[buf], b * 32 + (lane & 31), i * 16 + g * 8), kf[i], s);
@@ -360,12 +369,11 @@ __global__ __launch_bounds__(kNT, sizeof(T) == 2 ? 2 : 1) void attn_bwd_dkv_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x4 ls = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + 8 * i + 4 * g]);
-          const f32x4 de = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + 8 * i + 4 * g]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 4 * i + j;
             p[r] = __builtin_amdgcn_exp2f(s[r] * c - ls[j]);
-            s[r] = p[r] * (dp[r] - de[j]);
+            s[r] = p[r] * dp[r];
             if (kMasked && r0 + 8 * i + 4 * g + j < first) p[r] = s[r] = 0.0f;
           }
         }
