@@ -12,11 +12,13 @@
 // ones tiles in LDS that are read by rows for the products over channels and by columns for
 // those over rows.
 //
-// Bound: as the forward, the products (45 to 50 % of a SIMD's cycles) and the vector instructions
-// (30 to 40 %) one after the other; head size 128 also waits at its barriers, one each 32 rows.
-// Measured, dQ and dK/dV: 8,192 tokens, 16 x 64, bf16: 460 and 552 us, 900 and 1,000 TFLOP/s of the
-// three and four products done; packed causal sequences of 129 to 5,003 tokens, 16/4 x 128: 361 and
-// 505 us, 860 and 820; two fp32 clips of 2,048, 4 x 64: 130 and 154 us, 100 and 110.
+// Bound: products run in 46 to 52 % of a SIMD's cycles and vector instructions issue in 30 to 47 %;
+// two waves of 250 registers a SIMD do not fill the rest, waits for LDS and, at head size 128, for a
+// barrier each 32 rows.  dO V^T begins its sum with -delta, which spares a subtraction a weight (954
+// -> 934 us below).
+// Measured, dQ and dK/dV: 8,192 tokens, 16 x 64, bf16: 455 and 535 us, 910 and 1,030 TFLOP/s of the
+// three and four products done; packed causal sequences of 129 to 5,003 tokens, 16/4 x 128: 355 and
+// 480 us, 870 and 860; two fp32 clips of 2,048, 4 x 64: 130 and 154 us, 100 and 110.
 #include "attn_common.h"
 
 namespace msd {

@@ -8,10 +8,9 @@
 // fragment where it stands.  m is raised only where a score exceeds it by 2^8 or more in p
 // (p <= 256: nothing is lost in fp32), which spares most rescales.
 //
-// Bound: the matrix cores and the vector unit one after the other.  Of the cycles of a SIMD the
-// products take 45 % and the vector instructions 50 % (8,192 tokens, 16 x 64, bf16; 41 % and 35 %
-// at 16/4 heads x 128, causal), two to four waves a SIMD notwithstanding; LDS is busy for 20 %, and
-// nine in ten requests hit the L2.  Four waves of 32 rows and 64 keys: eight waves, or 32 keys,
+// Bound: the vector unit beside the matrix cores.  Of the cycles of a SIMD vector instructions issue
+// in 73 % and products run in 45 % (8,192 tokens, 16 x 64, bf16, four waves a SIMD; 46 % and 41 % at
+// 16/4 heads x 128, causal, two waves); LDS is busy for 20 %, and nine in ten requests hit the L2.  Four waves of 32 rows and 64 keys: eight waves, or 32 keys,
 // were 7 to 10 % slower, and so was the forward without the search for the maximum on the small
 // head sizes.  Tiles that a causal mask cuts are a loop of their own, so that the others compare
 // nothing.
@@ -248,7 +247,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
 // keys of the chunk for themselves and meet only at its end, so no wave waits for another.
 // A wave's next keys are on their way to LDS while it weighs the present values, and the next
 // values while it scores the next keys.  Parts are joined by attn_join_tokens_kernel.
-// 134,000 keys of 16 sequences, 32/8 heads x 128: 114 us, 4.8 TB/s (a copy reaches 5.1).
+// 131,000 keys of 16 sequences, 32/8 heads x 128: 112 us, 4.8 TB/s (a copy reaches 5.1), and 7
+// for the join; 119 with both launches.
 template <typename T, int HD>
 constexpr int kTokenWaves = sizeof(T) == 4 && HD > 64 ? 2 : 4;  // their tiles fill 64 KB of LDS
 
@@ -424,13 +424,17 @@ void attn_tokens_kernel(const AttnArgs a, T* __restrict__ out, T* __restrict__ r
 }
 
 // Joins the chunks of every sequence's first token, one workgroup a (row, head), its waves every
-// fourth chunk each; rows that no key belongs to (behind the last sequence, or of a sequence
-// without keys) become 0 and -inf.
+// eighth chunk each; rows that no key belongs to (behind the last sequence, or of a sequence
+// without keys) become 0 and -inf.  Bound: latency, of parts that other dies wrote: a wave has
+// eight of them on their way at a time (256 parts of 16 rows: 19 -> 7 us against four waves that
+// took them one after the other).
+constexpr int kJoinWaves = 8;
+
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_tokens_kernel(
+__global__ __launch_bounds__(kJoinWaves * 64) void attn_join_tokens_kernel(
     const AttnArgs a, const float* __restrict__ part, int chunk, int64_t units, int hd_padded,
     T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse) {
-  __shared__ float s_acc[4][128], s_sum[4];
+  __shared__ float s_acc[kJoinWaves][128], s_sum[kJoinWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.x / static_cast<unsigned>(a.hq);
   const int head = blockIdx.x - row * a.hq;
@@ -460,23 +464,37 @@ __global__ __launch_bounds__(256) void attn_join_tokens_kernel(
   for (int x = 32; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x));
   const float base = m == -INFINITY ? 0.0f : m;
   float sum = 0.0f, acc[2] = {0.0f, 0.0f};
-#pragma unroll 4
-  for (int k = wave; k < n; k += 4) {
-    const float w = exp2f((ls[k * step] - base) * kLog2e);
-    sum += w;
+  for (int k0 = wave; k0 < n; k0 += 8 * kJoinWaves) {
+    float w[8], v[8][2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (lane + 64 * x < a.hd) acc[x] += w * po[k * step * hd_padded + lane + 64 * x];
+    for (int u = 0; u < 8; ++u) {
+      const int k = k0 + u * kJoinWaves;
+      w[u] = k < n ? ls[k * step] : -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        v[u][x] = k < n && lane + 64 * x < a.hd ? po[k * step * hd_padded + lane + 64 * x] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float f = exp2f((w[u] - base) * kLog2e);
+      sum += f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) acc[x] += f * v[u][x];
+    }
   }
   s_acc[wave][lane] = acc[0];
   s_acc[wave][lane + 64] = acc[1];
   if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
-  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWaves; ++w) sum += s_sum[w];
   const int ch = threadIdx.x;
   const int64_t r = static_cast<int64_t>(row) * a.hq + head;
   if (ch < a.hd) {
-    float v = s_acc[0][ch] + s_acc[1][ch] + s_acc[2][ch] + s_acc[3][ch];
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) v += s_acc[w][ch];
     v = sum == 0.0f ? 0.0f : v / sum;
     out[r * a.hd + ch] = from_f32<T>(v);
     if (rest != nullptr) rest[r * a.hd + ch] = from_f32<T>(rest_of<T>(v));
@@ -535,7 +553,7 @@ hipError_t launch_tokens(const msd_attn_desc& d, const AttnArgs& a, T* out, T* r
           a, out, rest, lse, ws, chunk, units);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  attn_join_tokens_kernel<T><<<static_cast<unsigned>(a.total_q * a.hq), 256, 0, s>>>(
+  attn_join_tokens_kernel<T><<<static_cast<unsigned>(a.total_q * a.hq), kJoinWaves * 64, 0, s>>>(
       a, ws, chunk, units, HD, out, rest, lse);
   return hipGetLastError();
 }
