@@ -419,6 +419,49 @@ def test_streams_devices_and_graph():
                                                  new[4], causal=True))
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_single_tokens_in_graphs_and_on_two_streams(dt):
+    """Tokens over caches long enough to be joined from chunks: two captured graphs replayed in
+    turn with other lengths, and two calls at a time on two streams."""
+    from megaslide_amd import packed_attention
+    heads, kv, hd, total = 8, 2, 64, 3000
+    q, k, v, _ = inputs([1] * 3, [total], heads, kv, hd, dt)
+    cu = lens_to_cu([1, 1, 1], DEV)
+
+    def step(q, k, v, cu_k):
+        return packed_attention(q, k, v, heads, kv, cu, cu_k, True, return_lse=True)
+
+    static = [[t.clone() for t in (q, k, v, lens_to_cu([1000, 1000, 1000], DEV))]
+              for _ in range(2)]
+    graphs, res = [], []
+    for s in static:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            res.append(step(*s))
+    for seed, lens in ((41, [1000, 1000, 1000]), (42, [1, 2998, 1]), (43, [0, 17, 1500])):
+        new = []
+        for i, s in enumerate(static):
+            qi, ki, vi, _ = inputs([1] * 3, [total], heads, kv, hd, dt, seed + 10 * i)
+            new.append([qi, ki, vi, lens_to_cu(lens, DEV)])
+            for x, y in zip(s, new[-1]):
+                x.copy_(y)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for r, n in zip(res, new):
+            assert all(torch.equal(x, y) for x, y in zip(r, step(*n)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for st, n in zip(streams, new):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            got.append([step(*n) for _ in range(3)])
+    torch.cuda.synchronize()
+    for calls, n in zip(got, new):
+        want = step(*n)
+        assert all(torch.equal(x, y) for c in calls for x, y in zip(c, want))
+
+
 def test_offsets_out_of_order_stay_inside():
     """Offsets that break the documented order are held to the tensors' rows (their results are
     not defined): the calls end, and what follows on the same tensors is right."""
