@@ -17,9 +17,9 @@
 // the lane's own chunk (interleaved pairs) or read through LDS (pairs half an axis apart, which
 // no fixed shuffle serves for odd splits).  Where tokens are few, their heads are split among
 // workgroups.
-// Measured (a copy reaches 5.1 TB/s): rotation of 46,800 tokens, 16 x 96, bf16, 68 us forward and
-// 68 backward, 4.2 TB/s; with the norm, 65,536 tokens, 16 + 16 heads x 64, bf16, 131 and 190 us, 4.1
-// and 4.2 TB/s; 32,768 tokens, 8 + 8 x 64, fp32, 64 and 83 us, 4.2 and 4.8 TB/s; 16 tokens 6 us.
+// Measured (a copy reaches 5.1 TB/s): rotation of 46,800 tokens, 16 x 96, bf16, 65 us forward and
+// 65 backward, 4.4 TB/s; with the norm, 65,536 tokens, 16 + 16 heads x 64, bf16, 130 and 180 us, 4.1
+// and 4.5 TB/s; 32,768 tokens, 8 + 8 x 64, fp32, 64 and 83 us, 4.2 and 4.8 TB/s; 16 tokens 6 us.
 #include "common.h"
 #include "qk_rope.h"
 
@@ -124,7 +124,8 @@ __device__ __forceinline__ void load_weight(const void* p, int c0, int hd, float
   for (int i = 0; i < 8; ++i) v[i] = c0 + i < hd ? to_f32(static_cast<const T*>(p)[c0 + i]) : 0.0f;
 }
 
-template <typename T, bool VEC>
+// PAST: past the caches.
+template <typename T, bool VEC, bool PAST>
 __device__ __forceinline__ void store8(T* p, int c0, int hd, const float (&v)[8]) {
   if (VEC) {
     if (c0 >= hd) return;
@@ -133,7 +134,10 @@ __device__ __forceinline__ void store8(T* p, int c0, int hd, const float (&v)[8]
       bf16x8 r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = static_cast<__bf16>(v[i]);
-      *reinterpret_cast<bf16x8*>(p + c0) = r;
+      if constexpr (PAST)
+        __builtin_nontemporal_store(r, reinterpret_cast<bf16x8*>(p + c0));
+      else
+        *reinterpret_cast<bf16x8*>(p + c0) = r;
     } else {
       *reinterpret_cast<float4*>(p + c0) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(p + c0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -169,7 +173,7 @@ __device__ __forceinline__ float row_sum(float v, int sub, float* buf) {
 }
 
 // LPR: lanes of a row (8 channels each).
-template <typename T, int LPR, bool NORM, bool BWD, bool VEC, bool INTER>
+template <typename T, int LPR, bool NORM, bool BWD, bool VEC, bool INTER, bool PAST = false>
 __global__ __launch_bounds__(kThreads, 4) void qk_rope_kernel(const RopeArgs a) {
   constexpr int kRows = 64 / LPR;  // rows of a wave at a time (lanes behind them idle)
   constexpr int kAhead = sizeof(T) == 2 && !(NORM && BWD) ? 2 : 1;  // rows of a lane in flight
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(kThreads, 4) void qk_rope_kernel(const RopeArgs a) 
           for (int e = 0; e < 8; ++e) g[e] = r * g[e] - x[e] * f;
         }
         if (hh < h1 && grp < kRows)
-          store8<T, VEC>(ys + tok * out_stride + hh * hd, c0, hd, g);
+          store8<T, VEC, PAST>(ys + tok * out_stride + hh * hd, c0, hd, g);
       }
     }
   }
@@ -398,6 +402,19 @@ Shape grid_of(const msd_qk_rope_desc& d, bool bwd) {
 template <typename T, int LPR, bool NORM, bool BWD>
 void launch_vec(const RopeArgs& a, Shape g, bool vec, bool inter, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(g.x), g.y, a.heads[1] > 0 ? 2 : 1);
+  // Results of more than half the 256 MB behind the L2s go past the caches, where they would not
+  // stay until they are read (144 and 268 MB, forward and backward: 137 -> 133 and 310 -> 297 us; fp32,
+  // 134 MB: 152 -> 157, so in bf16 only).
+  if constexpr (sizeof(T) == 2) {
+    const int64_t values = a.tokens * (a.heads[0] + static_cast<int64_t>(a.heads[1])) * a.hd;
+    if (vec && values * 2 > (int64_t(128) << 20)) {
+      if (inter)
+        qk_rope_kernel<T, LPR, NORM, BWD, true, true, true><<<grid, kThreads, 0, s>>>(a);
+      else
+        qk_rope_kernel<T, LPR, NORM, BWD, true, false, true><<<grid, kThreads, 0, s>>>(a);
+      return;
+    }
+  }
   if (vec && inter) qk_rope_kernel<T, LPR, NORM, BWD, true, true><<<grid, kThreads, 0, s>>>(a);
   else if (vec) qk_rope_kernel<T, LPR, NORM, BWD, true, false><<<grid, kThreads, 0, s>>>(a);
   else if (inter) qk_rope_kernel<T, LPR, NORM, BWD, false, true><<<grid, kThreads, 0, s>>>(a);

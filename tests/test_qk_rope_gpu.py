@@ -217,6 +217,29 @@ def test_empty_and_nonfinite():
     assert torch.equal(yz, torch.zeros_like(yz)) and torch.isfinite(dz).all()
 
 
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("heads,kv,hd", [(16, 16, 64), (20, 4, 96), (9, 9, 128), (33, 33, 32)])
+def test_results_past_the_caches(heads, kv, hd, inter):
+    """Results of more than 128 MB are stored another way: the bits of calls on their parts."""
+    from megaslide_amd import qk_norm_rope
+    g = gen(12)
+    n = (135 << 20) // (2 * (heads + kv) * hd)
+    q, k, dq, dk = (randn(g, n, h * hd, dt=BF) for h in (heads, kv, heads, kv))
+    w = [randn(g, hd) for _ in range(2)]
+    pos = torch.randint(0, 500, (n, 3), generator=g, device=DEV, dtype=torch.int32)
+
+    def f(rows):
+        ins = [t[rows].requires_grad_(True) for t in (q, k)]
+        y = qk_norm_rope(*ins, *w, pos[rows], heads, kv, interleaved=inter)
+        return [t.detach() for t in y] + list(
+            torch.autograd.grad(y, ins, (dq[rows], dk[rows])))
+
+    whole = f(slice(None))
+    for rows in (slice(0, n // 2), slice(n // 2, n)):
+        for a, b in zip(whole, f(rows)):
+            assert torch.equal(a[rows], b)
+
+
 def test_saved_tensors_of_another_layout():
     """Hooks on saved tensors hand back contiguous copies of the views that were saved."""
     from megaslide_amd import qk_norm_rope
