@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -95,7 +95,8 @@ _NO_GRID = _Int3(0, 0, 0)
 
 
 class _RopeCall:
-    """Validated arguments of one rotation; ``args``: its C descriptor behind the strides."""
+    """Validated arguments of one rotation; ``head``, ``tail``: its C descriptor before and behind
+    the strides."""
 
     __slots__ = ("index", "weights", "pos", "head", "tail")
 
@@ -368,8 +369,8 @@ class _AttnCall:
         ws = q.new_empty(max(need, 16), dtype=torch.uint8)
         _lib.launch(lib.msd_attn_bwd, "attn_bwd", self.index, d, q.data_ptr(), self.k.data_ptr(),
                     self.v.data_ptr(), ptr(self.cu_q), ptr(self.cu_k), out.data_ptr(),
-                    ptr(rest), dout.data_ptr(), lse.data_ptr(), ptr(dlse), dq.data_ptr(), dk.data_ptr(),
-                    dv.data_ptr(), ws.data_ptr(), need)
+                    ptr(rest), dout.data_ptr(), lse.data_ptr(), ptr(dlse), dq.data_ptr(),
+                    dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need)
         return dq, dk, dv
 
 
